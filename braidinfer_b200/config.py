@@ -141,6 +141,9 @@ class Config:
     comm_timeout_s: float = 5.0
     heartbeat_every: int = 64      # TP: check peer liveness every N engine steps (0 = off)
     shared_prefix_batching: bool = True  # decode: attend once to segments shared by several sequences
+    kv_cache_dtype: str = "auto"   # "auto" (the model's dtype) | "int4" (ops/kv4.py: 72 instead of 256 bytes per 128 elements)
+    sliding_window: Optional[int] = None  # a token attends to this many last positions (its own included) ...
+    attention_sinks: int = 0       # ... and to the first so many positions of its composition
     validate_plans: bool = False   # check every step's metadata on the host before upload (also BRAID_VALIDATE_PLAN=1)
     seed: int = 0
     load_weights: bool = True     # False: random-init weights (synthetic benchmarks)
@@ -165,6 +168,19 @@ class Config:
             raise ConfigurationError("tensor_parallel_size must be 1, 2, 4 or 8")
         if self.comm_backend not in ("fused", "nccl"):
             raise ConfigurationError("comm_backend must be 'fused' or 'nccl'")
+        if self.kv_cache_dtype not in ("auto", "int4"):
+            raise ConfigurationError("kv_cache_dtype must be 'auto' or 'int4'")
+        if self.kv_cache_dtype == "int4":
+            if self.spec.head_dim not in (64, 128):
+                raise ConfigurationError(f"kv_cache_dtype 'int4' needs head_dim 64 or 128, got {self.spec.head_dim}")
+            if self.tensor_parallel_size != 1:
+                raise ConfigurationError("kv_cache_dtype 'int4' needs tensor_parallel_size 1")
+        if self.sliding_window is not None and not 1 <= self.sliding_window < 1 << 30:
+            raise ConfigurationError("sliding_window must be in [1, 2**30)")
+        if not 0 <= self.attention_sinks < 1 << 30:
+            raise ConfigurationError("attention_sinks must be in [0, 2**30)")
+        if self.attention_sinks and self.sliding_window is None:
+            raise ConfigurationError("attention_sinks needs a sliding_window")
 
     # -- resolved runtime properties ----------------------------------------
     @property

@@ -83,6 +83,7 @@ class ModelRunner:
         else:
             self.model.random_init(seed=config.seed, std=config.init_std, k_norm_range=config.init_k_norm_range)
         self.model.finalize()
+        self.model.window, self.model.sinks = config.sliding_window or 0, config.attention_sinks
         log.info("model ready in %.1fs", time.time() - t0)
         self.page_manager: Optional[PageManager] = None
         self.page_size = config.kvcache_block_size
@@ -107,8 +108,11 @@ class ModelRunner:
     # ------------------------------------------------------------- KV pool
     def kv_bytes_per_page(self) -> int:
         L = self.model.layout
-        return 2 * self.spec.num_layers * L.kv_heads * self.page_size * self.spec.head_dim * \
-            torch.tensor([], dtype=self.dtype).element_size()
+        if self.config.kv_cache_dtype == "int4":
+            row = ops.KV4Cache.row_bytes(self.spec.head_dim)
+        else:
+            row = self.spec.head_dim * torch.tensor([], dtype=self.dtype).element_size()
+        return 2 * self.spec.num_layers * L.kv_heads * self.page_size * row
 
     def auto_num_pages(self) -> int:
         cfg = self.config
@@ -133,7 +137,7 @@ class ModelRunner:
         L = self.model.layout
         n = self.auto_num_pages()
         self.page_manager = PageManager(n, self.page_size, self.spec.num_layers, L.kv_heads, self.spec.head_dim,
-                                        self.dtype, self.device)
+                                        self.dtype, self.device, int4=self.config.kv_cache_dtype == "int4")
         log.info("KV pool: %d pages x %d tokens (%.2f GB)", n, self.page_size,
                  n * self.kv_bytes_per_page() / 1e9)
         return self.page_manager
@@ -237,7 +241,8 @@ class ModelRunner:
         """Reorder a decode batch so a shared-prefix group comes first; returns
         ``(seqs, items, group)`` (``group`` None when no segment is shared)."""
         items = self._items_for(seqs)
-        if not self.config.shared_prefix_batching or len(seqs) < 2 or not hasattr(self.model, "layout"):
+        if not self.config.shared_prefix_batching or len(seqs) < 2 or not hasattr(self.model, "layout") or \
+                self.model.window or self.page_manager.int4:  # the windowed and 4-bit kernels take no group
             return seqs, items, None
         found = find_shared_group(items, self.page_size)
         if found is None:

@@ -26,12 +26,13 @@ import numpy as np
 import torch
 
 from ..errors import OutOfPagesError
+from ..ops.kv4 import KV4Cache
 from .sequence import Sequence
 
 
 class PageManager:
     def __init__(self, num_pages: int, page_size: int, num_layers: int, num_kv_heads: int, head_dim: int,
-                 dtype: torch.dtype, device: torch.device):
+                 dtype: torch.dtype, device: torch.device, int4: bool = False):
         if num_pages < 2:
             raise OutOfPagesError("KV pool needs at least 2 pages")
         self.num_pages = num_pages
@@ -40,8 +41,12 @@ class PageManager:
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.dtype = dtype
-        self.kv_cache = torch.zeros(num_layers, num_pages, 2, num_kv_heads, page_size, head_dim,
-                                    dtype=dtype, device=device)
+        self.int4 = int4
+        if int4:  # the same pages and slots, 4-bit content (ops/kv4.py)
+            self.kv_cache = KV4Cache(num_layers, num_pages, num_kv_heads, page_size, head_dim, device=device)
+        else:
+            self.kv_cache = torch.zeros(num_layers, num_pages, 2, num_kv_heads, page_size, head_dim,
+                                        dtype=dtype, device=device)
         self.scratch_page = num_pages - 1
         self.refcount = np.zeros(num_pages, dtype=np.int32)
         self.refcount[self.scratch_page] = 1 << 30
@@ -56,7 +61,8 @@ class PageManager:
     # ---------------------------------------------------------------- basics
     @property
     def bytes_per_page(self) -> int:
-        return 2 * self.num_layers * self.num_kv_heads * self.page_size * self.head_dim * self.kv_cache.element_size()
+        row = KV4Cache.row_bytes(self.head_dim) if self.int4 else self.head_dim * self.kv_cache.element_size()
+        return 2 * self.num_layers * self.num_kv_heads * self.page_size * row
 
     @property
     def num_free_pages(self) -> int:

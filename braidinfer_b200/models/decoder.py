@@ -102,6 +102,7 @@ class DecoderLM:
         else:
             self.cos = self.sin = torch.zeros(1, max(1, D // 2), device=device)
         self.scale = 1.0 / math.sqrt(D)
+        self.window, self.sinks = 0, 0  # sliding window (0: none) and its sinks, set by the runner
         # ERNIE: interleaved rotary pairs -> neox half split by a row permutation.
         self.rope_perm = None
         if spec.family == "ernie":
@@ -266,7 +267,8 @@ class DecoderLM:
             gu_done = nxt(w.gu_w, T)
             if PREFETCH_ATTN and not PREFETCH_ALL:
                 ops.prefetch_next(w.o_w, T)
-            o = ops.attention(q, kv_cache[i], meta, self.cos, self.sin, self.scale, S.use_rope, workspace)
+            o = ops.attention(q, kv_cache[i], meta, self.cos, self.sin, self.scale, S.use_rope, workspace,
+                              self.window, self.sinks)
             residual = self._row_parallel(o, w.o_w, residual, w.gu_w, gu_done)
             nxt(w.down_w, T)
             g = ops.linear_swiglu(residual, w.gu_w, rms_eps=eps)
@@ -294,7 +296,8 @@ class DecoderLM:
             q = ops.qkv_gemm(G, w.qkv_w, w.qkv_b, eps, positions, slot_mapping, kv_cache[i], L.q_heads,
                              L.kv_heads, S.head_dim, self.cos, self.sin, w.q_norm, w.k_norm, eps, S.use_rope,
                              rs_vec=rstd, sp=fc.sp_params())
-            o = ops.attention(q, kv_cache[i], meta, self.cos, self.sin, self.scale, S.use_rope, workspace)
+            o = ops.attention(q, kv_cache[i], meta, self.cos, self.sin, self.scale, S.use_rope, workspace,
+                              self.window, self.sinks)
             fc.sp_linear_reduce_scatter(o.view(o.shape[0], -1), w.o_w, G)
             fc.sp_reduce_allgather(eps)
             g = ops.linear_swiglu(G, w.gu_w, rms_eps=eps, rs_vec=rstd, sp=fc.sp_params())

@@ -47,6 +47,7 @@ class GPT2LM:
         self.lm_head = self.embed
         self.cos = self.sin = torch.zeros(1, max(1, D // 2), device=device)
         self.scale = 1.0 / math.sqrt(D)
+        self.window, self.sinks = 0, 0  # sliding window (0: none) and its sinks, set by the runner
 
     def random_init(self, seed: int = 0, std: float = 0.02, k_norm_range=None) -> None:
         g = torch.Generator(device=self.device)
@@ -132,7 +133,8 @@ class GPT2LM:
             qkv = ops.linear(x, w["qkv_w"], w["qkv_b"])
             q = ops.qkv_prepare(qkv, positions, slot_mapping, kv_cache[i], L.q_heads, L.q_heads, S.head_dim,
                                 self.cos, self.sin, None, None, eps, False)
-            o = ops.attention(q, kv_cache[i], meta, self.cos, self.sin, self.scale, False, workspace)
+            o = ops.attention(q, kv_cache[i], meta, self.cos, self.sin, self.scale, False, workspace,
+                              self.window, self.sinks)
             if self.tp.size == 1:
                 h = ops.linear(o, w["o_w"], w["o_b"], residual=h)
             else:

@@ -18,6 +18,13 @@ private segment and inside a chunk's own prefill, and full visibility of every
 earlier chunk — the cascade of ``braidinfer/layers/cascade_attention.py:50-231``
 without its per-page Python loop.
 
+With ``window`` W > 0 it must also hold that ``p - (seg_pos0[s] + j) < W`` or
+``seg_pos0[s] + j < sinks``: the last W positions (the query's own among them)
+and the first ``sinks`` positions of the composition.  A query that sees no key
+gets zeros.  Slots that no query of a tile sees may hold anything, NaN included.
+
+The cache may also be a 4-bit one (``kv4.KV4Layer``): same pages, slots and plan.
+
 Queries are stored *unrotated*; the kernel rotates them by ``p - seg_delta[s]``
 per segment (differential RoPE on the query side, O(|Q|) per chunk instead of
 re-rotating O(|K|) cached keys).
@@ -25,11 +32,12 @@ re-rotating O(|K|) cached keys).
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
 from ._ext import ext
+from .kv4 import KV4Layer, kv4_pack_ref, kv4_unpack_ref
 from .norm import rms_norm_ref
 from .rope import apply_rope_ref
 
@@ -66,7 +74,7 @@ class AttnMeta:
 
 
 def qkv_prepare(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
-                kv_layer: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                kv_layer: Union[torch.Tensor, KV4Layer], num_q_heads: int, num_kv_heads: int, head_dim: int,
                 cos: torch.Tensor, sin: torch.Tensor, q_norm: Optional[torch.Tensor] = None,
                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, use_rope: bool = True) -> torch.Tensor:
     """Split ``qkv[T, (Hq+2Hkv)*D]``; per-head q/k RMSNorm (Qwen3); RoPE on k;
@@ -74,8 +82,17 @@ def qkv_prepare(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.
 
     Replaces the reference's per-token ``.item()`` append loop
     (``braidinfer/kernels/kv_cache_utils.py:9-78``) with one kernel.
+
+    Into a :class:`KV4Layer` the norm, RoPE and codes are computed in fp32 from
+    the bf16 input (no rounding in between), and without a ``q_norm`` the
+    returned q is a view of ``qkv``.  The slots of one call must differ, unless
+    what they hold is never read (padding); on CUDA a slot outside the cache is
+    skipped.
     """
     T = qkv.shape[0]
+    if isinstance(kv_layer, KV4Layer):
+        return _qkv_prepare_kv4(qkv, positions, slot_mapping, kv_layer, num_q_heads, num_kv_heads, head_dim, cos, sin,
+                                q_norm, k_norm, eps, use_rope)
     if qkv.is_cuda:
         q = torch.empty(T, num_q_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
         ext().qkv_prepare(q, qkv, positions, slot_mapping, kv_layer, q_norm, k_norm, float(eps), cos, sin,
@@ -98,8 +115,34 @@ def qkv_prepare(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.
     return q.contiguous()
 
 
+def _qkv_prepare_kv4(qkv, positions, slot_mapping, kv_layer, num_q_heads, num_kv_heads, head_dim, cos, sin, q_norm,
+                     k_norm, eps, use_rope):
+    T = qkv.shape[0]
+    codes, scales = kv_layer
+    qs = num_q_heads * head_dim
+    view = qkv[:, :qs].unflatten(1, (num_q_heads, head_dim))
+    if qkv.is_cuda:
+        q = view if q_norm is None else torch.empty(T, num_q_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
+        ext().qkv_prepare_kv4(q, qkv, positions, slot_mapping, codes, scales, q_norm, k_norm, float(eps), cos, sin,
+                              num_q_heads, num_kv_heads, head_dim, bool(use_rope))
+        return q
+
+    def norm(x, w):
+        return x if w is None else x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+
+    kv = qkv[:, qs:].float().unflatten(1, (2, num_kv_heads, head_dim))
+    k = norm(kv[:, 0], k_norm)
+    if use_rope:
+        k = apply_rope_ref(k, positions, cos, sin)
+    c, sc = kv4_pack_ref(torch.stack([k, kv[:, 1]], 1))
+    slots, ps = slot_mapping.long(), kv_layer.page_size
+    codes[slots // ps, :, :, slots % ps] = c
+    scales[slots // ps, :, :, slots % ps] = sc
+    return view if q_norm is None else norm(view.float(), q_norm).to(qkv.dtype)
+
+
 def qkv_gemm(x: torch.Tensor, w_qkv: torch.Tensor, bias: Optional[torch.Tensor], rms_eps: Optional[float],
-             positions: torch.Tensor, slot_mapping: torch.Tensor, kv_layer: torch.Tensor, num_q_heads: int,
+             positions: torch.Tensor, slot_mapping: torch.Tensor, kv_layer: Union[torch.Tensor, KV4Layer], num_q_heads: int,
              num_kv_heads: int, head_dim: int, cos: torch.Tensor, sin: torch.Tensor,
              q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
              use_rope: bool = True, rs_vec: Optional[torch.Tensor] = None,
@@ -108,8 +151,16 @@ def qkv_gemm(x: torch.Tensor, w_qkv: torch.Tensor, bias: Optional[torch.Tensor],
     folded into ``w_qkv``) with the q/k-norm, RoPE(k) and paged KV append done
     in the GEMM epilogue on CUDA.  Returns unrotated q ``[T, Hq, D]``.
     ``rs_vec``/``sp``: precomputed ``1/rms`` and sequence-parallel parameters
-    (CUDA tensor-parallel prefill)."""
+    (CUDA tensor-parallel prefill).  Into a :class:`KV4Layer` the projection and
+    ``qkv_prepare`` are two launches; ``rs_vec``/``sp`` are refused there."""
     T = x.shape[0]
+    if isinstance(kv_layer, KV4Layer):
+        if rs_vec is not None or sp is not None:
+            raise ValueError("qkv_gemm: a 4-bit cache takes no precomputed 1/rms and no sequence-parallel parameters")
+        from .linear import linear
+
+        return qkv_prepare(linear(x, w_qkv, bias, rms_eps=rms_eps), positions, slot_mapping, kv_layer, num_q_heads,
+                           num_kv_heads, head_dim, cos, sin, q_norm, k_norm, eps, use_rope)
     if x.is_cuda:
         q = torch.empty(T, num_q_heads, head_dim, dtype=x.dtype, device=x.device)
         ext().gemm_qkv(q, x, w_qkv, bias, -1.0 if rms_eps is None else float(rms_eps), positions, slot_mapping,
@@ -123,12 +174,14 @@ def qkv_gemm(x: torch.Tensor, w_qkv: torch.Tensor, bias: Optional[torch.Tensor],
                        q_norm, k_norm, eps, use_rope)
 
 
-def attention_ref(q: torch.Tensor, kv_layer: torch.Tensor, meta: AttnMeta, cos: torch.Tensor,
-                  sin: torch.Tensor, scale: float, use_rope: bool = True) -> torch.Tensor:
-    """fp32 restatement of the cascade kernel (one softmax over all segments)."""
+def attention_ref(q: torch.Tensor, kv_layer: Union[torch.Tensor, KV4Layer], meta: AttnMeta, cos: torch.Tensor,
+                  sin: torch.Tensor, scale: float, use_rope: bool = True, window: int = 0,
+                  sinks: int = 0) -> torch.Tensor:
+    """fp32 restatement of the cascade kernels (one softmax over all segments)."""
     h = meta.host
     T, Hq, D = q.shape
-    P, _, Hkv, page, _ = kv_layer.shape
+    q4 = isinstance(kv_layer, KV4Layer)
+    _, _, Hkv, page, _ = kv_layer.codes.shape if q4 else kv_layer.shape
     G = Hq // Hkv
     out = torch.zeros(T, Hq, D, dtype=torch.float32)
     qo, segp = h["qo_indptr"], h["seg_indptr"]
@@ -151,8 +204,12 @@ def attention_ref(q: torch.Tensor, kv_layer: torch.Tensor, meta: AttnMeta, cos: 
             slot = int(h["seg_offset"][s]) + torch.arange(n)
             pg = pages[slot // page]
             off = slot % page
-            k = kv_layer[pg, 0, :, off, :].float()  # [n, Hkv, D]
-            v = kv_layer[pg, 1, :, off, :].float()
+            if q4:
+                kv = kv4_unpack_ref(kv_layer.codes[pg, :, :, off], kv_layer.scales[pg, :, :, off])
+                k, v = kv[:, 0], kv[:, 1]
+            else:
+                k = kv_layer[pg, 0, :, off, :].float()  # [n, Hkv, D]
+                v = kv_layer[pg, 1, :, off, :].float()
             qq = q[t0:t1].float()
             if use_rope:
                 qq = apply_rope_ref(qq, pos - int(h["seg_delta"][s]), cos, sin)
@@ -160,6 +217,8 @@ def attention_ref(q: torch.Tensor, kv_layer: torch.Tensor, meta: AttnMeta, cos: 
             sc = torch.einsum("thd,nhd->htn", qq, kk) * scale
             kpos = int(h["seg_pos0"][s]) + torch.arange(n)
             mask = kpos[None, :] > pos[:, None]  # [t, n]
+            if window > 0:
+                mask = mask | ((pos[:, None] - kpos[None, :] >= window) & (kpos[None, :] >= sinks))
             sc = sc.masked_fill(mask[None], float("-inf"))
             scores.append(sc)
             values.append(v.repeat_interleave(G, dim=1))
@@ -173,11 +232,33 @@ def attention_ref(q: torch.Tensor, kv_layer: torch.Tensor, meta: AttnMeta, cos: 
     return out.to(q.dtype).reshape(T, Hq * D)
 
 
-def attention(q: torch.Tensor, kv_layer: torch.Tensor, meta: AttnMeta, cos: torch.Tensor, sin: torch.Tensor,
-              scale: float, use_rope: bool = True, workspace: Optional[dict] = None) -> torch.Tensor:
+def attention(q: torch.Tensor, kv_layer: Union[torch.Tensor, KV4Layer], meta: AttnMeta, cos: torch.Tensor,
+              sin: torch.Tensor, scale: float, use_rope: bool = True, workspace: Optional[dict] = None,
+              window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """Attention of ``q [T, Hq, D]`` over the plan's segments -> ``[T, Hq * D]``
+    (the masking rule, ``window`` and ``sinks``: module text; ``window`` 0 is no
+    window, and ``sinks`` without one changes nothing).
+
+    A :class:`KV4Layer` or a window takes its own kernels
+    (``csrc/attention_rows.cu``): decode or not follows from the rows, keys are
+    split inside the kernel without a workspace, ``meta.num_splits`` is not
+    used, and a plan with a shared-prefix group is refused."""
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0 or window >= 1 << 30 or sinks >= 1 << 30:
+        raise ValueError(f"attention: window and sinks must be in [0, 2**30), got {window} and {sinks}")
+    q4 = isinstance(kv_layer, KV4Layer)
+    if (q4 or window > 0) and meta.seq_nsh is not None:
+        raise ValueError("attention: a shared-prefix plan takes neither a 4-bit cache nor a window")
     if q.is_cuda:
         T, Hq, D = q.shape
         out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
+        if q4 or window > 0:
+            kv, scales = kv_layer if q4 else (kv_layer, None)
+            ext().attention_rows(out, q, kv, scales, meta.qo_indptr, meta.positions, meta.seg_indptr,
+                                 meta.seg_page_indptr, meta.seg_offset, meta.seg_len, meta.seg_pos0, meta.seg_delta,
+                                 meta.page_ids, cos, sin, float(scale), bool(use_rope), int(meta.num_seqs),
+                                 int(meta.max_q_len), int(meta.max_kv_len), window, sinks)
+            return out
         ws = workspace or {}
         ext().attention(out, q, kv_layer, meta.qo_indptr, meta.positions, meta.seg_indptr,
                         meta.seg_page_indptr, meta.seg_offset, meta.seg_len, meta.seg_pos0, meta.seg_delta,
@@ -186,4 +267,4 @@ def attention(q: torch.Tensor, kv_layer: torch.Tensor, meta: AttnMeta, cos: torc
                         ws.get("partial_o"), ws.get("partial_lse"), meta.grp_qo_indptr, meta.grp_seg_indptr,
                         meta.seq_nsh, int(meta.shared_splits), int(meta.grp_max_q))
         return out
-    return attention_ref(q, kv_layer, meta, cos, sin, scale, use_rope)
+    return attention_ref(q, kv_layer, meta, cos, sin, scale, use_rope, window, sinks)

@@ -25,25 +25,36 @@ from .parallel.state import get_tp
 MANIFEST = "chunks.json"
 
 
+def _tensors(pm) -> Dict[str, torch.Tensor]:
+    """The KV pool's tensors ``[L, P, 2, Hkv, page, ...]`` by the suffix of their key in the file: the pool itself, or
+    the codes and scales of a 4-bit one (saved as they are held, without a second rounding)."""
+    return {"": pm.kv_cache.codes, ".scales": pm.kv_cache.scales} if pm.int4 else {"": pm.kv_cache}
+
+
 def fingerprint(cl) -> str:
     eng = cl.llm
     spec = eng.config.spec
     tp = get_tp()
-    desc = json.dumps({"spec": {k: v for k, v in spec.__dict__.items() if k not in ("eos_token_id", "bos_token_id")},
-                       "dtype": str(eng.model_runner.dtype), "tp": tp.size, "page": eng.page_manager.page_size},
-                      sort_keys=True, default=str)
+    cfg = eng.config
+    what = {"spec": {k: v for k, v in spec.__dict__.items() if k not in ("eos_token_id", "bos_token_id")},
+            "dtype": str(eng.model_runner.dtype), "tp": tp.size, "page": eng.page_manager.page_size}
+    if cfg.kv_cache_dtype != "auto":
+        what["kv"] = cfg.kv_cache_dtype
+    if cfg.sliding_window is not None:  # a chunk's KV depends on what its own tokens attended to
+        what["window"] = [cfg.sliding_window, cfg.attention_sinks]
+    desc = json.dumps(what, sort_keys=True, default=str)
     return hashlib.sha256(desc.encode()).hexdigest()
 
 
-def _gather(pm, chunk: Chunk) -> torch.Tensor:
+def _gather(pm, chunk: Chunk) -> Dict[str, torch.Tensor]:
     ps = pm.page_size
     slots = torch.arange(chunk.kv_offset, chunk.kv_offset + chunk.kv_length)
     pages = torch.tensor(chunk.page_table, dtype=torch.long)[slots // ps]
     off = slots % ps
     dev = pm.kv_cache.device
     # advanced indices separated by slices put the token dim first: [n, L, 2, Hkv, D]
-    kv = pm.kv_cache[:, pages.to(dev), :, :, off.to(dev), :]
-    return kv.permute(1, 2, 3, 0, 4).contiguous().cpu()      # [L, 2, Hkv, n, D]
+    return {sfx: t[:, pages.to(dev), :, :, off.to(dev)].movedim(0, 3).contiguous().cpu()  # [L, 2, Hkv, n, ...]
+            for sfx, t in _tensors(pm).items()}
 
 
 def save_chunks(cl, path: str) -> int:
@@ -61,7 +72,7 @@ def save_chunks(cl, path: str) -> int:
                                "cached_position_start": c.cached_position_start, "kv_length": 0,
                                "cascade_level": c.cascade_level}
         if c.kv_cache_allocated and c.page_table and c.kv_length:
-            tensors[c.chunk_id] = _gather(pm, c)
+            tensors.update({c.chunk_id + sfx: t for sfx, t in _gather(pm, c).items()})
             rec["kv_length"] = c.kv_length
             if c.last_hidden is not None:
                 tensors[c.chunk_id + ".last_hidden"] = c.last_hidden.detach().float().cpu().contiguous()
@@ -94,14 +105,14 @@ def load_chunks(cl, path: str) -> int:
         n += 1
         if rec["kv_length"] == 0 or c.kv_cache_allocated or sf is None:
             continue
-        kv = sf.get_tensor(cid)  # [L, 2, Hkv, n, D]
         pages = pm.allocate_for_chunk(cid, rec["kv_length"])
         ps = pm.page_size
         slots = torch.arange(rec["kv_length"])
         dev = pm.kv_cache.device
         pg = torch.tensor(pages, dtype=torch.long)[slots // ps].to(dev)
         off = (slots % ps).to(dev)
-        pm.kv_cache[:, pg, :, :, off, :] = kv.permute(3, 0, 1, 2, 4).to(dev, pm.kv_cache.dtype)
+        for sfx, t in _tensors(pm).items():
+            t[:, pg, :, :, off] = sf.get_tensor(cid + sfx).movedim(3, 0).to(dev, t.dtype)  # [n, L, 2, Hkv, ...]
         c.page_table, c.kv_length, c.kv_offset = pages, rec["kv_length"], 0
         c.cached_position_start = rec["cached_position_start"]
         c.cascade_level = rec["cascade_level"]

@@ -15,6 +15,8 @@ unsigned long long bounds_status_gemm();
 unsigned long long bounds_status_gemm_persistent();
 unsigned long long bounds_status_attention();
 unsigned long long bounds_status_attention_tc();
+unsigned long long bounds_status_attention_rows();
+unsigned long long bounds_status_kv4();
 unsigned long long bounds_status_elementwise();
 unsigned long long bounds_status_sampling();
 unsigned long long bounds_status_comm();
@@ -23,7 +25,7 @@ unsigned long long bounds_status_comm();
 // checked build: code << 48 | value; every file's word is read and cleared.
 int64_t bounds_check_status() {
   unsigned long long first = 0;
-  for (auto fn : {bounds_status_gemm, bounds_status_gemm_persistent, bounds_status_attention, bounds_status_attention_tc, bounds_status_elementwise, bounds_status_sampling, bounds_status_comm}) {
+  for (auto fn : {bounds_status_gemm, bounds_status_gemm_persistent, bounds_status_attention, bounds_status_attention_tc, bounds_status_attention_rows, bounds_status_kv4, bounds_status_elementwise, bounds_status_sampling, bounds_status_comm}) {
     const unsigned long long v = fn();
     if (first == 0) first = v;
   }
@@ -71,6 +73,17 @@ void attention(torch::Tensor out, torch::Tensor q, torch::Tensor kv, torch::Tens
                c10::optional<torch::Tensor> part_o, c10::optional<torch::Tensor> part_lse,
                c10::optional<torch::Tensor> grp_qo_indptr, c10::optional<torch::Tensor> grp_seg_indptr,
                c10::optional<torch::Tensor> seq_nsh, int64_t shared_splits, int64_t grp_max_q);
+void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::optional<torch::Tensor> scales,
+                    torch::Tensor qo_indptr, torch::Tensor positions, torch::Tensor seg_indptr,
+                    torch::Tensor seg_page_indptr, torch::Tensor seg_offset, torch::Tensor seg_len,
+                    torch::Tensor seg_pos0, torch::Tensor seg_delta, torch::Tensor page_ids, torch::Tensor cos,
+                    torch::Tensor sin, double scale, bool use_rope, int64_t num_seqs, int64_t max_q_len,
+                    int64_t max_kv_len, int64_t window, int64_t sinks);
+void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor slots,
+                     torch::Tensor codes, torch::Tensor scales, c10::optional<torch::Tensor> q_norm,
+                     c10::optional<torch::Tensor> k_norm, double eps, torch::Tensor cos, torch::Tensor sin,
+                     int64_t Hq, int64_t Hkv, int64_t D, bool use_rope);
+void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torch::Tensor slots);
 void attn_set_trace(torch::Tensor buf);
 void attn_tc_set_trace(torch::Tensor buf);
 void attn_select_prefill_tc(int64_t mode);
@@ -140,6 +153,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("decode"), py::arg("num_splits"), py::arg("part_o") = py::none(), py::arg("part_lse") = py::none(),
         py::arg("grp_qo_indptr") = py::none(), py::arg("grp_seg_indptr") = py::none(),
         py::arg("seq_nsh") = py::none(), py::arg("shared_splits") = 0, py::arg("grp_max_q") = 0);
+  m.def("attention_rows", &braid::attention_rows,
+        "paged cascade attention of few rows over a bf16 or 4-bit cache, with an optional window and sinks");
+  m.def("qkv_prepare_kv4", &braid::qkv_prepare_kv4, "q/k norm, RoPE(k) and append to the 4-bit paged cache");
+  m.def("kv4_read", &braid::kv4_read, "the values a 4-bit cache holds at the given slots");
   m.def("attn_prefill_tile_rows", &braid::attn_prefill_tile_rows,
         "query rows per CTA of the prefill attention kernel for head_dim D (256: tcgen05, one CTA per SM; 64: mma.sync, two)");
   m.def("attn_set_exp2_poly", &braid::attn_set_exp2_poly,

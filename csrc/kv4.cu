@@ -1,0 +1,285 @@
+// Append to and read-back from the 4-bit paged KV cache (layout in kv4.cuh).
+//
+// qkv_prepare_kv4: one pass over a step's QKV rows: per-head q/k RMSNorm,
+// RoPE(k), per-group minimum and maximum, codes and scales stored at the
+// token's slot.  Everything from the bf16 input to the code is fp32; the only
+// roundings are those the format defines and, for a normalised q, one to bf16.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "common.cuh"
+#include "kv4.cuh"
+#include "launch.cuh"
+
+namespace braid {
+
+unsigned long long* next_span(const char* name);
+
+struct Kv4AppendParams {
+  const __nv_bfloat16* qkv;  // [T, ld] rows of (Hq + 2 Hkv) heads
+  __nv_bfloat16* q_out;      // [T, Hq, D], written only with a q norm
+  uint32_t* codes;           // layer codes as words
+  uint32_t* scales;          // layer (s, z) pairs
+  const int* positions;
+  const int* slots;
+  const __nv_bfloat16* qn;   // nullptr: no norm
+  const __nv_bfloat16* kn;
+  const float* cos;
+  const float* sin;
+  float eps;
+  int64_t ld;
+  int64_t items;             // T * heads handled
+  int heads;                 // handled per token: 2 Hkv, or Hq + 2 Hkv with a q norm
+  int Hq, Hkv, PS, use_rope, num_slots, rope_len;
+  unsigned long long* span;
+};
+
+// D / 8 lanes per (token, head), 8 elements (one 16-byte load, one code word)
+// per lane; the rotary partner of a lane's elements is D / 16 lanes away, and
+// 8 neighbouring lanes hold one group of 64.  Lanes past the last item stay
+// for the shuffles and touch no memory.
+template <int D>
+__global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendParams p) {
+  constexpr int LPH = D / 8;
+  if (threadIdx.x == 0) span_start(p.span);
+  pdl_trigger();
+  pdl_wait();
+  if (threadIdx.x == 0) span_waited(p.span);
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  const int l = threadIdx.x % LPH;
+  const bool live = item < p.items;
+  const int64_t t = live ? item / p.heads : 0;
+  const int head = (int)(live ? item % p.heads : 0) + (p.Hq + 2 * p.Hkv - p.heads);  // within the QKV row
+  const bool is_q = head < p.Hq, is_k = !is_q && head < p.Hq + p.Hkv;
+  float v[8];
+  {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (live) u = *reinterpret_cast<const uint4*>(p.qkv + t * p.ld + (int64_t)head * D + l * 8);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    }
+  }
+  const __nv_bfloat16* nw = is_q ? p.qn : (is_k ? p.kn : nullptr);
+  {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (nw != nullptr) {
+      const float rstd = rsqrtf(ss / D + p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * bf2f(nw[l * 8 + j]);
+    }
+  }
+  if (is_q && live) {
+    uint4 o = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    *reinterpret_cast<uint4*>(p.q_out + (t * p.Hq + head) * D + l * 8) = o;
+  }
+  {
+    float partner[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) partner[j] = __shfl_xor_sync(0xffffffffu, v[j], LPH / 2);
+    if (is_k && p.use_rope && live) {
+      int pos = p.positions[t];
+      (void)BRAID_IN_BOUNDS(pos >= 0 && pos < p.rope_len, 2, pos);
+      pos = min(max(pos, 0), p.rope_len - 1);
+      const bool first = l < LPH / 2;
+      const int64_t at = (int64_t)pos * (D / 2) + (l % (LPH / 2)) * 8;
+      float cs[8], sn[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        *reinterpret_cast<float4*>(cs + j) = *reinterpret_cast<const float4*>(p.cos + at + j);
+        *reinterpret_cast<float4*>(sn + j) = *reinterpret_cast<const float4*>(p.sin + at + j);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = first ? v[j] * cs[j] - partner[j] * sn[j] : v[j] * cs[j] + partner[j] * sn[j];
+    }
+  }
+  float mn = v[0], mx = v[0], bad = v[0] - v[0];  // bad: 0, or NaN once an element is not finite
+#pragma unroll
+  for (int j = 1; j < 8; ++j) {
+    mn = fminf(mn, v[j]);
+    mx = fmaxf(mx, v[j]);
+    bad += v[j] - v[j];
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    bad += __shfl_xor_sync(0xffffffffu, bad, o);
+  }
+  const int slot = live ? p.slots[t] : -1;
+  if (live && !is_q && BRAID_IN_BOUNDS(slot >= 0 && slot < p.num_slots, 1, slot) && slot >= 0 && slot < p.num_slots) {
+    // mx - mn passes the fp32 range only for values of magnitude above 1.7e38; such a group counts as not finite
+    const float range = mx - mn;
+    const bool fine = bad == 0.f && range <= 3.4e38f;
+    const __nv_bfloat16 sb = f2bf(fine ? __fdiv_rn(range, 15.f) : __int_as_float(0x7fc00000));
+    const __nv_bfloat16 zb = f2bf(fine ? mn : __int_as_float(0x7fc00000));
+    const float s = bf2f(sb), z = bf2f(zb);
+    uint32_t word = 0;
+    if (fine && s > 0.f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(v[j] - z, s)), 0.f), 15.f);
+        word |= (uint32_t)c << (4 * j);
+      }
+    }
+    const int page = slot / p.PS, off = slot % p.PS;
+    const int kh = is_k ? head - p.Hq : head - p.Hq - p.Hkv;
+    const int64_t row = (((int64_t)page * 2 + (is_k ? 0 : 1)) * p.Hkv + kh) * p.PS + off;
+    p.codes[row * (D / 8) + kv4_word<D>(l)] = word;
+    if (l % 8 == 0)
+      p.scales[row * (D / KV4_GROUP) + l / 8] =
+          (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+  }
+  if (threadIdx.x == 0) span_end(p.span);
+}
+
+// out[t, kv, head, :] = the values held at slots[t]; zeros for a slot outside the cache.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* __restrict__ out,
+                                                       const uint32_t* __restrict__ codes,
+                                                       const uint32_t* __restrict__ scales,
+                                                       const int* __restrict__ slots, int64_t items, int Hkv, int PS,
+                                                       int num_slots) {
+  constexpr int LPH = D / 8;
+  pdl_trigger();
+  pdl_wait();
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  const int l = threadIdx.x % LPH;
+  if (item >= items) return;
+  const int64_t t = item / (2 * Hkv);
+  const int kvh = (int)(item % (2 * Hkv));
+  const int slot = slots[t];
+  uint4 o = make_uint4(0, 0, 0, 0);
+  if (BRAID_IN_BOUNDS(slot >= 0 && slot < num_slots, 1, slot) && slot >= 0 && slot < num_slots) {
+    const int64_t row = ((int64_t)(slot / PS) * 2 * Hkv + kvh) * PS + slot % PS;
+    const uint32_t w = codes[row * (D / 8) + kv4_word<D>(l)];
+    const uint32_t sz = scales[row * (D / KV4_GROUP) + l / 8];
+    const float s = kv4_scale(sz), z = kv4_offset(sz);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = fmaf(s, (float)((w >> (4 * j)) & 15u), z);
+    o = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  }
+  *reinterpret_cast<uint4*>(out + item * D + l * 8) = o;
+}
+
+// ------------------------------------------------------------------ host
+void kv4_check_layer(const torch::Tensor& codes, const torch::Tensor& scales, const char* who) {
+  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.dim() == 5 && codes.is_contiguous(), who,
+              ": 4-bit cache codes must be a contiguous CUDA uint8 tensor [P, 2, Hkv, page, D/2]");
+  TORCH_CHECK(scales.is_cuda() && scales.scalar_type() == at::kBFloat16 && scales.dim() == 6 && scales.is_contiguous(),
+              who, ": 4-bit cache scales must be a contiguous CUDA bf16 tensor [P, 2, Hkv, page, D/64, 2]");
+  TORCH_CHECK(scales.device() == codes.device(), who, ": codes and scales on different devices");
+  const int64_t D = codes.size(4) * 2;
+  TORCH_CHECK(D == 64 || D == 128, who, ": 4-bit cache head_dim must be 64 or 128");
+  TORCH_CHECK(codes.size(1) == 2 && scales.size(0) == codes.size(0) && scales.size(1) == 2 &&
+                  scales.size(2) == codes.size(2) && scales.size(3) == codes.size(3) &&
+                  scales.size(4) == D / KV4_GROUP && scales.size(5) == 2,
+              who, ": 4-bit cache codes and scales do not match");
+  TORCH_CHECK(codes.size(0) * codes.size(3) < (1ll << 31), who, ": more than 2^31 slots");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 8 == 0,
+              who, ": 4-bit cache tensors must be 16-byte (codes) and 8-byte (scales) aligned");
+}
+
+static void check_i32(const torch::Tensor& t, int64_t n, const torch::Device& dev, const char* who, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == dev && t.numel() >= n, who, ": ", name,
+              " must be a contiguous int32 tensor of at least ", std::to_string(n), " elements on the device of the cache");
+}
+
+void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor slots,
+                     torch::Tensor codes, torch::Tensor scales, c10::optional<torch::Tensor> q_norm,
+                     c10::optional<torch::Tensor> k_norm, double eps, torch::Tensor cos, torch::Tensor sin,
+                     int64_t Hq, int64_t Hkv, int64_t D, bool use_rope) {
+  const char* who = "qkv_prepare";
+  kv4_check_layer(codes, scales, who);
+  const auto dev = codes.device();
+  TORCH_CHECK(qkv.is_cuda() && qkv.device() == dev && qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 &&
+                  qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(1) == 1 && qkv.stride(0) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+              who, ": qkv must be a bf16 [T, (Hq + 2 Hkv) D] tensor with 16-byte aligned rows on the device of the cache");
+  TORCH_CHECK(codes.size(2) == Hkv && codes.size(4) * 2 == D, who, ": cache layout mismatch");
+  const int64_t T = qkv.size(0);
+  if (T == 0) return;
+  check_i32(positions, T, dev, who, "positions");
+  check_i32(slots, T, dev, who, "slots");
+  const bool has_qn = q_norm.has_value() && q_norm->defined(), has_kn = k_norm.has_value() && k_norm->defined();
+  for (const auto* w : {has_qn ? &*q_norm : nullptr, has_kn ? &*k_norm : nullptr})
+    if (w != nullptr)
+      TORCH_CHECK(w->device() == dev && w->scalar_type() == at::kBFloat16 && w->numel() == D && w->is_contiguous(), who,
+                  ": norm weights must be contiguous bf16 [D] on the device of the cache");
+  if (use_rope)
+    TORCH_CHECK(cos.device() == dev && sin.device() == dev && cos.scalar_type() == at::kFloat &&
+                    sin.scalar_type() == at::kFloat && cos.is_contiguous() && sin.is_contiguous() && cos.dim() == 2 &&
+                    cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes(),
+                who, ": cos and sin must be contiguous fp32 [positions, D/2] tables on the device of the cache");
+  if (has_qn)
+    TORCH_CHECK(q_out.device() == dev && q_out.scalar_type() == at::kBFloat16 && q_out.is_contiguous() &&
+                    q_out.numel() == T * Hq * D,
+                who, ": q_out must be a contiguous bf16 [T, Hq, D] tensor");
+  const at::cuda::CUDAGuard g(dev);
+  Kv4AppendParams p{};
+  p.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
+  p.q_out = has_qn ? reinterpret_cast<__nv_bfloat16*>(q_out.data_ptr()) : nullptr;
+  p.codes = reinterpret_cast<uint32_t*>(codes.data_ptr());
+  p.scales = reinterpret_cast<uint32_t*>(scales.data_ptr());
+  p.positions = positions.data_ptr<int>();
+  p.slots = slots.data_ptr<int>();
+  p.qn = has_qn ? reinterpret_cast<const __nv_bfloat16*>(q_norm->data_ptr()) : nullptr;
+  p.kn = has_kn ? reinterpret_cast<const __nv_bfloat16*>(k_norm->data_ptr()) : nullptr;
+  p.cos = use_rope ? cos.data_ptr<float>() : nullptr;
+  p.sin = use_rope ? sin.data_ptr<float>() : nullptr;
+  p.eps = (float)eps;
+  p.ld = qkv.stride(0);
+  p.heads = (int)(2 * Hkv + (has_qn ? Hq : 0));
+  p.items = T * p.heads;
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.PS = (int)codes.size(3);
+  p.use_rope = use_rope ? 1 : 0;
+  p.num_slots = (int)(codes.size(0) * codes.size(3));
+  p.rope_len = use_rope ? (int)cos.size(0) : 1;
+  p.span = next_span("qkv_prepare_kv4");
+  const int64_t per_block = 256 / (D / 8);
+  const dim3 grid((unsigned)((p.items + per_block - 1) / per_block));
+  auto st = at::cuda::getCurrentCUDAStream();
+  if (D == 128)
+    launch_pdl(qkv_prepare_kv4_kernel<128>, grid, dim3(256), 0, st, p);
+  else
+    launch_pdl(qkv_prepare_kv4_kernel<64>, grid, dim3(256), 0, st, p);
+}
+
+void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torch::Tensor slots) {
+  const char* who = "kv4_read";
+  kv4_check_layer(codes, scales, who);
+  const int64_t T = slots.numel(), Hkv = codes.size(2), PS = codes.size(3), D = codes.size(4) * 2;
+  if (T == 0) return;
+  check_i32(slots, T, codes.device(), who, "slots");
+  TORCH_CHECK(out.device() == codes.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
+                  out.numel() == T * 2 * Hkv * D,
+              who, ": out must be a contiguous bf16 [T, 2, Hkv, D] tensor");
+  const at::cuda::CUDAGuard g(codes.device());
+  const int64_t items = T * 2 * Hkv, per_block = 256 / (D / 8);
+  const dim3 grid((unsigned)((items + per_block - 1) / per_block));
+  auto st = at::cuda::getCurrentCUDAStream();
+  auto* o = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  const auto* c = reinterpret_cast<const uint32_t*>(codes.data_ptr());
+  const auto* s = reinterpret_cast<const uint32_t*>(scales.data_ptr());
+  if (D == 128)
+    launch_pdl(kv4_read_kernel<128>, grid, dim3(256), 0, st, o, c, s, (const int*)slots.data_ptr<int>(), items, (int)Hkv,
+               (int)PS, (int)(codes.size(0) * PS));
+  else
+    launch_pdl(kv4_read_kernel<64>, grid, dim3(256), 0, st, o, c, s, (const int*)slots.data_ptr<int>(), items, (int)Hkv,
+               (int)PS, (int)(codes.size(0) * PS));
+}
+
+BRAID_BOUNDS_READER(bounds_status_kv4)
+
+}  // namespace braid
