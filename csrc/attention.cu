@@ -1169,6 +1169,7 @@ void attention(torch::Tensor out, torch::Tensor q, torch::Tensor kv, torch::Tens
   p.scale_log2 = (float)scale * LOG2E;
   p.use_rope = use_rope ? 1 : 0;
   p.Hq = Hq;
+  p.q_stride = (int64_t)Hq * D;
   p.Hkv = Hkv;
   p.G = G;
   p.PS = PS;

@@ -29,6 +29,11 @@
 // with num_splits > 1 each CTA covers one range of the visible keys and the
 // last CTA of the q tile merges (log-sum-exp); partial_only publishes the
 // partials for the decode kernel (shared-prefix decode).
+// WIN instances (a call with a window, or over a 4-bit cache read into a
+// workspace) walk two intervals per segment, the sink part and the window part
+// of what the CTA's rows see, so keys behind every row's window are not loaded;
+// V rows outside the interval are zeroed before P V (P is 0 there, but the slots
+// may hold NaN).
 // Replaces the reference's per-page Triton online-softmax calls
 // (braidinfer/kernels/online_softmax.py:15-214) on the prefill side.
 #include <torch/extension.h>
@@ -92,24 +97,49 @@ struct TcWalk {
 
 struct TcRange {
   int max_pos, r0, r1;
+  int min_pos;  // WIN
 };
 
 BRAID_DEVICE int tc_seg_vis(const AttnParams& p, int s, int max_pos) {
   return max(0, min(p.seg_len[s], max_pos - p.seg_pos0[s] + 1));
 }
 
-// Advance w to the next segment with keys in [r0, r1); false when done.
+// The walk's index w.s counts segments, with WIN twice: 2 segment + part.
+template <bool WIN>
+BRAID_DEVICE int tc_seg(int s) {
+  return WIN ? s >> 1 : s;
+}
+// Keys [a, b) that index s stands for: those some row of the CTA can see; with
+// WIN the sink part (first positions of the composition) and the window part.
+template <bool WIN>
+BRAID_DEVICE void tc_interval(const AttnParams& p, const TcRange& rg, int s, int& a, int& b) {
+  const int vis = tc_seg_vis(p, tc_seg<WIN>(s), rg.max_pos);
+  a = 0;
+  b = vis;
+  if (WIN) {
+    const int pos0 = p.seg_pos0[s >> 1];
+    int wlo = min(max(rg.min_pos - p.window + 1 - pos0, 0), vis);
+    int slo = min(max(p.sinks - pos0, 0), vis);
+    if (slo >= wlo) wlo = slo = 0;  // they meet: one interval
+    a = (s & 1) ? wlo : 0;
+    b = (s & 1) ? vis : slo;
+  }
+}
+
+// Advance w to the next interval with keys in [r0, r1); false when done.
+template <bool WIN>
 BRAID_DEVICE bool tc_settle(const AttnParams& p, const TcRange& rg, TcWalk& w) {
   while (w.s < w.s1) {
-    const int vis = tc_seg_vis(p, w.s, rg.max_pos);
-    w.lo = max(0, rg.r0 - w.segstart);
-    w.hi = min(vis, rg.r1 - w.segstart);
+    int a, b;
+    tc_interval<WIN>(p, rg, w.s, a, b);
+    w.lo = a + max(0, rg.r0 - w.segstart);
+    w.hi = WIN ? (b - a <= rg.r1 - w.segstart ? b : a + (rg.r1 - w.segstart)) : min(b, rg.r1 - w.segstart);
     if (w.lo < w.hi) {
-      w.off = p.seg_offset[w.s];
+      w.off = p.seg_offset[tc_seg<WIN>(w.s)];
       w.sl = (w.off + w.lo) & ~(TC_KEYS - 1);
       return true;
     }
-    w.segstart += vis;
+    w.segstart += WIN ? max(b - a, 0) : b;
     ++w.s;
   }
   return false;
@@ -117,14 +147,19 @@ BRAID_DEVICE bool tc_settle(const AttnParams& p, const TcRange& rg, TcWalk& w) {
 
 // Next tile; returns false when the walk is over.  *new_seg is set when the
 // next tile belongs to a different segment than the current one.
+template <bool WIN>
 BRAID_DEVICE bool tc_next(const AttnParams& p, const TcRange& rg, TcWalk& w, bool* new_seg) {
   w.sl += TC_KEYS;
   *new_seg = false;
   if (w.sl < w.off + w.hi) return true;
-  w.segstart += tc_seg_vis(p, w.s, rg.max_pos);
+  const int was = tc_seg<WIN>(w.s);
+  int a, b;
+  tc_interval<WIN>(p, rg, w.s, a, b);
+  w.segstart += WIN ? max(b - a, 0) : b;
   ++w.s;
-  *new_seg = true;
-  return tc_settle(p, rg, w);
+  const bool more = tc_settle<WIN>(p, rg, w);
+  *new_seg = !WIN || tc_seg<WIN>(w.s) != was;
+  return more;
 }
 
 // Rotated query row r (token tok, head) for a segment with RoPE delta `delta`,
@@ -133,7 +168,7 @@ BRAID_DEVICE bool tc_next(const AttnParams& p, const TcRange& rg, TcWalk& w, boo
 // halves of 16 float4 loads each (about three memory round trips per row).
 BRAID_DEVICE void tc_build_q_row(const AttnParams& p, uint8_t* qs, int r, bool live, int tok, int head, int rpos,
                                  int delta) {
-  const __nv_bfloat16* qp = p.q + ((size_t)tok * p.Hq + head) * TC_D;
+  const __nv_bfloat16* qp = p.q + (size_t)tok * p.q_stride + (size_t)head * TC_D;
   uint4 qa[8], qb[8];
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
@@ -221,7 +256,7 @@ BRAID_DEVICE float tc_exp2_poly(float x) {
 }
 
 // POLY: every POLY-th exponential of a row runs tc_exp2_poly (0: none).
-template <int BR, int POLY>
+template <int BR, int POLY, bool WIN>
 __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmkv,
                                                                         const AttnParams p) {
   extern __shared__ uint8_t sm_raw[];
@@ -265,13 +300,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     rg.max_pos = mx;
+    if (WIN) {
+      int mn = INT_MAX;
+      for (int tk = ta + lane; tk <= tb; tk += 32) mn = min(mn, p.positions[tk]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      rg.min_pos = max(mn, 0);
+    }
   }
-  const int s0 = p.seg_indptr[b], s1 = p.seg_indptr[b + 1];
+  const int s0 = p.seg_indptr[b] * (WIN ? 2 : 1), s1 = p.seg_indptr[b + 1] * (WIN ? 2 : 1);
   rg.r0 = 0;
   rg.r1 = 1 << 30;
   if (S > 1) {
     int total = 0;
-    for (int s = s0; s < s1; ++s) total += tc_seg_vis(p, s, rg.max_pos);
+    for (int s = s0; s < s1; ++s) {
+      int a, e;
+      tc_interval<WIN>(p, rg, s, a, e);
+      total += max(e - a, 0);
+    }
     const int per = ((total + S - 1) / S + TC_KEYS - 1) / TC_KEYS * TC_KEYS;
     rg.r0 = min(total, split * per);
     rg.r1 = min(total, rg.r0 + per);
@@ -305,7 +351,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
   if (trc != nullptr && threadIdx.x == 0) trc[126] = globaltimer_ns();
 
   TcWalk w{s0, s1, 0, 0, 0, 0, 0};
-  bool more = tc_settle(p, rg, w);
+  bool more = tc_settle<WIN>(p, rg, w);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -316,13 +362,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
       while (more) {
         const int st = j % TC_STAGES;
         const uint32_t ph = ((j / TC_STAGES) & 1) ^ 1;
-        const int* pages = p.page_ids + p.seg_page_indptr[w.s];
-        const int npages = p.seg_page_indptr[w.s + 1] - p.seg_page_indptr[w.s];
+        const int page0 = p.seg_page_indptr[tc_seg<WIN>(w.s)];
+        const int* pages = p.page_ids + page0;
+        const int npages = p.seg_page_indptr[tc_seg<WIN>(w.s) + 1] - page0;
         int rk[TC_KEYS / BR];
 #pragma unroll
         for (int q = 0; q < TC_KEYS / BR; ++q) {
           const int slot = w.sl + q * BR;
-          const int page = pages[min(slot / p.PS, npages - 1)];
+          const int idx = min(slot / p.PS, npages - 1);
+          const int page = WIN && p.page_identity ? page0 + idx : pages[idx];
           (void)BRAID_IN_BOUNDS(page >= 0 && page < p.num_pages, 4, page);  // TMA zero-fills outside the pool
           rk[q] = ((page * 2 + 0) * p.Hkv + kh) * p.PS + slot % p.PS;
         }
@@ -351,7 +399,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
                         rk[q] + p.Hkv * p.PS);
         ++viss;
         bool ns;
-        more = tc_next(p, rg, w, &ns);
+        more = tc_next<WIN>(p, rg, w, &ns);
         ++j;
       }
       // every copy this CTA issued lands before the CTA can finish (a consumer
@@ -399,7 +447,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
       while (ok) {
         const int st = j % TC_STAGES, st1 = (j + 1) % TC_STAGES;
         bool ns;
-        const bool nxt = tc_next(p, rg, w, &ns);
+        const bool nxt = tc_next<WIN>(p, rg, w, &ns);
         if (!mbar_wait(&bar.vfull[st], (j / TC_STAGES) & 1)) {
           ok = false;
           break;
@@ -451,7 +499,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
       float m_run = -INFINITY, l_run = 0.f;
       int j = 0;
       if (more) {
-        const int delta0 = p.seg_delta[w.s];
+        const int delta0 = p.seg_delta[tc_seg<WIN>(w.s)];
         pdl_wait();
         tc_build_q_row(p, qs, r, live, tok, head, rpos, delta0);
         fence_proxy_async_smem();
@@ -459,7 +507,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
         if (trc != nullptr && r == 0) trc[t * 64 + 60] = globaltimer_ns();
       }
       while (more) {
-        const int pos0 = p.seg_pos0[w.s], j0 = w.sl - w.off, lo = w.lo, hi = w.hi;
+        const int pos0 = p.seg_pos0[tc_seg<WIN>(w.s)], j0 = w.sl - w.off, lo = w.lo, hi = w.hi;
         if (!mbar_wait(&bar.sfull[t], j & 1)) {
           s_abort = 1;
           break;
@@ -472,11 +520,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
         tc_wait_ld();
         // keys outside [lo, hi) of the segment, or after the row's position,
         // are masked; interior tiles (every key visible to this row) skip it
-        if (live && !(j0 >= lo && j0 + TC_KEYS <= hi && pos0 + j0 + TC_KEYS - 1 <= rpos)) {
+        // (with WIN also keys behind the row's window that are not sinks)
+        if (live && !(j0 >= lo && j0 + TC_KEYS <= hi && pos0 + j0 + TC_KEYS - 1 <= rpos &&
+                      (!WIN || pos0 + j0 > rpos - p.window || pos0 + j0 + TC_KEYS <= p.sinks))) {
 #pragma unroll
           for (int i = 0; i < TC_KEYS; ++i) {
             const int key = j0 + i;
-            if (!(key >= lo && key < hi && pos0 + key <= rpos)) sr[i] = __float_as_uint(-INFINITY);
+            if (!(key >= lo && key < hi && pos0 + key <= rpos &&
+                  (!WIN || pos0 + key > rpos - p.window || pos0 + key < p.sinks)))
+              sr[i] = __float_as_uint(-INFINITY);
+          }
+        }
+        // V rows outside the interval (row r of the tile is key j0 + r) become zero before this tile's P V
+        if (WIN && t == 0 && (j0 < lo || j0 + TC_KEYS > hi)) {
+          const int st = j % TC_STAGES;
+          if (!mbar_wait(&bar.vfull[st], (j / TC_STAGES) & 1)) {
+            s_abort = 1;
+            break;
+          }
+          if (j0 + r < lo || j0 + r >= hi) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              *reinterpret_cast<uint4*>(vst + st * TC_TILE + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(vst + st * TC_TILE + TC_HALF + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            }
           }
         }
         // eight independent partial maxima (a 128-long dependent chain otherwise)
@@ -527,10 +594,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
         }
         tc_wait_st();
         bool ns;
-        more = tc_next(p, rg, w, &ns);
+        more = tc_next<WIN>(p, rg, w, &ns);
         // S(t, j) is consumed and S(t, j + 1) waits for this arrival: the next
         // segment's rotated queries can replace the Q tile now
-        if (more && ns) tc_build_q_row(p, qs, r, live, tok, head, rpos, p.seg_delta[w.s]);
+        if (more && ns) tc_build_q_row(p, qs, r, live, tok, head, rpos, p.seg_delta[tc_seg<WIN>(w.s)]);
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(&bar.pready[t]);
@@ -700,23 +767,28 @@ void launch_attn_prefill_tc(const AttnParams& p, int num_seqs, int max_q_len, in
   }();
   const int poly = g_attn_poly >= 0 ? g_attn_poly : env_poly;
   auto go = [&](auto k, int br) {
-    static bool attr[8] = {};
-    const int slot = (br == 64 ? 4 : 0) + (poly == 2 ? 1 : poly == 4 ? 2 : 0);
+    static bool attr[16] = {};
+    const int slot = (br == 64 ? 4 : 0) + (p.window > 0 ? 8 : poly == 2 ? 1 : poly == 4 ? 2 : 0);
     if (!attr[slot]) {
       C10_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem::TOTAL));
       attr[slot] = true;
     }
     launch_pdl(k, grid, dim3(TC_THREADS), TcSmem::TOTAL, st, make_tmap(p.kv, rows, TC_D, TC_D, br), p);
   };
-  if (p.PS % 64 == 0) {
-    if (poly == 2)
-      go(attn_prefill_tc_kernel<64, 2>, 64);
-    else if (poly == 4)
-      go(attn_prefill_tc_kernel<64, 4>, 64);
+  if (p.window > 0) {
+    if (p.PS % 64 == 0)
+      go(attn_prefill_tc_kernel<64, 0, true>, 64);
     else
-      go(attn_prefill_tc_kernel<64, 0>, 64);
+      go(attn_prefill_tc_kernel<16, 0, true>, 16);
+  } else if (p.PS % 64 == 0) {
+    if (poly == 2)
+      go(attn_prefill_tc_kernel<64, 2, false>, 64);
+    else if (poly == 4)
+      go(attn_prefill_tc_kernel<64, 4, false>, 64);
+    else
+      go(attn_prefill_tc_kernel<64, 0, false>, 64);
   } else {
-    go(attn_prefill_tc_kernel<16, 0>, 16);
+    go(attn_prefill_tc_kernel<16, 0, false>, 16);
   }
 }
 

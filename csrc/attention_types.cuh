@@ -49,6 +49,10 @@ struct AttnParams {
   int split_stride;           // partial slots per (token, head); 0: num_splits
   int split_base;             // first slot of this launch's splits
   int partial_only;           // prefill kernel: publish partials, do not merge
+  int64_t q_stride;           // tcgen05 prefill: elements between the q rows of two tokens
+  int window;                 // tcgen05 prefill: positions a query sees back from its own (0: no window) ...
+  int sinks;                  // ... and the first positions it always sees
+  int page_identity;          // tcgen05 prefill: page i of the plan's list is page i of the pool
   const int* seq_nsh;         // decode: 1 for sequences of the shared-prefix group (nullptr: none)
 };
 

@@ -190,6 +190,13 @@ BRAID_DEVICE void tma_load_2d(void* smem_dst, const void* desc, uint64_t* bar, i
       ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(smem_u32(bar)), "r"(x), "r"(y)
       : "memory");
 }
+// The same with a shared-memory address.
+BRAID_DEVICE void tma_load_2d_u32(uint32_t smem_dst, const void* desc, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(desc)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
 
 // L2 cache policy for streams read exactly once (decode weights, this step's
 // K/V): evicted first, so they do not push out lines other kernels prefetched.

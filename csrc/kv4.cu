@@ -8,6 +8,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include "attention_rows.cuh"
 #include "common.cuh"
 #include "kv4.cuh"
 #include "launch.cuh"
@@ -140,12 +141,22 @@ __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendPar
   if (threadIdx.x == 0) span_end(p.span);
 }
 
+// Values 8 l .. 8 l + 7 of a cache row as bf16.
+template <int D>
+BRAID_DEVICE uint4 kv4_values(const uint32_t* codes, const uint32_t* scales, int64_t row, int l) {
+  const uint32_t w = codes[row * (D / 8) + kv4_word<D>(l)];
+  const uint32_t sz = scales[row * (D / KV4_GROUP) + l / 8];
+  const float s = kv4_scale(sz), z = kv4_offset(sz);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = fmaf(s, (float)((w >> (4 * j)) & 15u), z);
+  return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
 // out[t, kv, head, :] = the values held at slots[t]; zeros for a slot outside the cache.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* __restrict__ out,
-                                                       const uint32_t* __restrict__ codes,
-                                                       const uint32_t* __restrict__ scales,
-                                                       const int* __restrict__ slots, int64_t items, int Hkv, int PS,
+__global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* out, const uint32_t* codes,
+                                                       const uint32_t* scales, const int* slots, int64_t items, int Hkv, int PS,
                                                        int num_slots) {
   constexpr int LPH = D / 8;
   pdl_trigger();
@@ -159,18 +170,77 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* __restrict
   uint4 o = make_uint4(0, 0, 0, 0);
   if (BRAID_IN_BOUNDS(slot >= 0 && slot < num_slots, 1, slot) && slot >= 0 && slot < num_slots) {
     const int64_t row = ((int64_t)(slot / PS) * 2 * Hkv + kvh) * PS + slot % PS;
-    const uint32_t w = codes[row * (D / 8) + kv4_word<D>(l)];
-    const uint32_t sz = scales[row * (D / KV4_GROUP) + l / 8];
-    const float s = kv4_scale(sz), z = kv4_offset(sz);
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fmaf(s, (float)((w >> (4 * j)) & 15u), z);
-    o = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    o = kv4_values<D>(codes, scales, row, l);
   }
   *reinterpret_cast<uint4*>(out + item * D + l * 8) = o;
 }
 
+// Page i of the plan's list as bf16 page i of `out` [NP, 2, Hkv, PS, D], for the long-prompt attention: the slots of its
+// segment that some query of the sequence sees (the others, which may hold anything, become 0).  Pages that no query
+// sees are skipped: the attention does not read them.  One block per (page, K/V and head).
+template <int D>
+__global__ void __launch_bounds__(256) kv4_unpack_pages_kernel(__nv_bfloat16* out, const RowsParams p,
+                                                               int num_seqs) {
+  constexpr int LPR = D / 8;
+  __shared__ int s_seg, s_seq, s_min, s_max;
+  const int i = blockIdx.x;
+  if (threadIdx.x == 0) {
+    s_seg = s_seq = -1;
+    s_min = INT_MAX;
+    s_max = -1;
+  }
+  pdl_trigger();
+  pdl_wait();
+  __syncthreads();
+  const int segs = p.seg_indptr[num_seqs];
+  for (int s = threadIdx.x; s < segs; s += 256)
+    if (p.seg_page_indptr[s] <= i && i < p.seg_page_indptr[s + 1]) s_seg = s;
+  __syncthreads();
+  const int s = s_seg;
+  if (s < 0) return;
+  for (int b = threadIdx.x; b < num_seqs; b += 256)
+    if (p.seg_indptr[b] <= s && s < p.seg_indptr[b + 1]) s_seq = b;
+  __syncthreads();
+  if (s_seq < 0) return;
+  int mn = INT_MAX, mx = -1;
+  for (int t = p.qo_indptr[s_seq] + threadIdx.x; t < p.qo_indptr[s_seq + 1]; t += 256) {
+    mn = min(mn, p.positions[t]);
+    mx = max(mx, p.positions[t]);
+  }
+  mn = __reduce_min_sync(0xffffffffu, mn);
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMin(&s_min, mn);
+    atomicMax(&s_max, mx);
+  }
+  __syncthreads();
+  const int off = p.seg_offset[s], len = p.seg_len[s], pos0 = p.seg_pos0[s];
+  const int slot0 = (i - p.seg_page_indptr[s]) * p.PS;  // of the segment's pages
+  // keys of this page, and those of them that lie in front of every query's window and behind the sinks or after them all
+  const int a = max(slot0 - off, 0), b = min(slot0 + p.PS - off, len);
+  if (a >= b || pos0 + a > s_max) return;
+  if (p.window > 0 && pos0 + b - 1 <= s_min - p.window && pos0 + a >= p.sinks) return;
+  const int page = min(max(p.page_ids[i], 0), p.num_pages - 1);
+  (void)BRAID_IN_BOUNDS(p.page_ids[i] >= 0 && p.page_ids[i] < p.num_pages, 4, p.page_ids[i]);
+  const int kvh = blockIdx.y;
+  const int64_t src = ((int64_t)page * 2 * p.Hkv + kvh) * p.PS, dst = ((int64_t)i * 2 * p.Hkv + kvh) * p.PS;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.kv);
+  for (int e = threadIdx.x; e < p.PS * LPR; e += 256) {
+    const int r = e / LPR, l = e % LPR;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (slot0 + r - off >= a && slot0 + r - off < b) o = kv4_values<D>(codes, p.scales, src + r, l);
+    *reinterpret_cast<uint4*>(out + (dst + r) * D + l * 8) = o;
+  }
+}
+
 // ------------------------------------------------------------------ host
+void kv4_unpack_pages(torch::Tensor out, const torch::Tensor& codes, const torch::Tensor& scales, const RowsParams& p,
+                      int64_t num_seqs, cudaStream_t st) {
+  TORCH_CHECK(codes.size(4) == 64 && out.is_contiguous() && out.scalar_type() == at::kBFloat16, "attention: unpack");
+  launch_pdl(kv4_unpack_pages_kernel<128>, dim3((unsigned)out.size(0), (unsigned)(2 * p.Hkv)), dim3(256), 0, st,
+             reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), p, (int)num_seqs);
+}
+
 void kv4_check_layer(const torch::Tensor& codes, const torch::Tensor& scales, const char* who) {
   TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.dim() == 5 && codes.is_contiguous(), who,
               ": 4-bit cache codes must be a contiguous CUDA uint8 tensor [P, 2, Hkv, page, D/2]");
@@ -185,8 +255,8 @@ void kv4_check_layer(const torch::Tensor& codes, const torch::Tensor& scales, co
               who, ": 4-bit cache codes and scales do not match");
   TORCH_CHECK(codes.size(0) * codes.size(3) < (1ll << 31), who, ": more than 2^31 slots");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 8 == 0,
-              who, ": 4-bit cache tensors must be 16-byte (codes) and 8-byte (scales) aligned");
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+              who, ": 4-bit cache tensors must be 16-byte aligned");
 }
 
 static void check_i32(const torch::Tensor& t, int64_t n, const torch::Device& dev, const char* who, const char* name) {

@@ -136,6 +136,8 @@ def tolerance(out, A, B, q_eps, p_eps, kv_eps=0.0):
 # what each kernel rounds: (queries, P, K and V)
 ROWS4 = (2 ** -11, 2 ** -11, 0.0)   # fp16 queries and P, exact codes
 ROWS16 = (2 ** -16, 2 ** -8, 0.0)   # queries as two bf16 terms, bf16 P
+TC16 = (2 ** -8, 2 ** -8, 0.0)      # long prompts: bf16 queries and P ...
+TC4 = (2 ** -8, 2 ** -8, 2 ** -8)   # ... and a 4-bit cache read into bf16
 
 
 def check(got, ref, eps, what=""):
