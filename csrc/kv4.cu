@@ -16,6 +16,7 @@
 namespace braid {
 
 unsigned long long* next_span(const char* name);
+int gemm_num_sms();
 
 struct Kv4AppendParams {
   const __nv_bfloat16* qkv;  // [T, ld] rows of (Hq + 2 Hkv) heads
@@ -30,149 +31,177 @@ struct Kv4AppendParams {
   const float* sin;
   float eps;
   int64_t ld;
-  int64_t items;             // T * heads handled
-  int heads;                 // handled per token: 2 Hkv, or Hq + 2 Hkv with a q norm
+  unsigned items;            // T * heads handled
+  unsigned heads;            // handled per token: 2 Hkv, or Hq + 2 Hkv with a q norm
   int Hq, Hkv, PS, use_rope, num_slots, rope_len;
   unsigned long long* span;
 };
 
+BRAID_DEVICE void unpack8(uint4 u, float* v) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(w[j] << 16);
+    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+BRAID_DEVICE uint4 pack8(const float* v) {
+  return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
 // D / 8 lanes per (token, head), 8 elements (one 16-byte load, one code word)
 // per lane; the rotary partner of a lane's elements is D / 16 lanes away, and
-// 8 neighbouring lanes hold one group of 64.  Lanes past the last item stay
-// for the shuffles and touch no memory.
-template <int D>
+// 8 neighbouring lanes hold one group of 64.  U items per thread, all loads of
+// them issued first.  Lanes past the last item stay for the shuffles and touch
+// no memory.
+template <int D, int U>
 __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendParams p) {
-  constexpr int LPH = D / 8;
+  constexpr int LPH = D / 8, IPB = 256 / LPH;
   if (threadIdx.x == 0) span_start(p.span);
   pdl_trigger();
   pdl_wait();
   if (threadIdx.x == 0) span_waited(p.span);
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
   const int l = threadIdx.x % LPH;
-  const bool live = item < p.items;
-  const int64_t t = live ? item / p.heads : 0;
-  const int head = (int)(live ? item % p.heads : 0) + (p.Hq + 2 * p.Hkv - p.heads);  // within the QKV row
-  const bool is_q = head < p.Hq, is_k = !is_q && head < p.Hq + p.Hkv;
-  float v[8];
-  {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (live) u = *reinterpret_cast<const uint4*>(p.qkv + t * p.ld + (int64_t)head * D + l * 8);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  const unsigned first = blockIdx.x * (IPB * U) + threadIdx.x / LPH;
+  unsigned tok[U];
+  int head[U], slot[U], pos[U];
+  uint4 raw[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-    }
-  }
-  const __nv_bfloat16* nw = is_q ? p.qn : (is_k ? p.kn : nullptr);
-  {
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (nw != nullptr) {
-      const float rstd = rsqrtf(ss / D + p.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * bf2f(nw[l * 8 + j]);
-    }
-  }
-  if (is_q && live) {
-    uint4 o = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    *reinterpret_cast<uint4*>(p.q_out + (t * p.Hq + head) * D + l * 8) = o;
-  }
-  {
-    float partner[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) partner[j] = __shfl_xor_sync(0xffffffffu, v[j], LPH / 2);
-    if (is_k && p.use_rope && live) {
-      int pos = p.positions[t];
-      (void)BRAID_IN_BOUNDS(pos >= 0 && pos < p.rope_len, 2, pos);
-      pos = min(max(pos, 0), p.rope_len - 1);
-      const bool first = l < LPH / 2;
-      const int64_t at = (int64_t)pos * (D / 2) + (l % (LPH / 2)) * 8;
-      float cs[8], sn[8];
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        *reinterpret_cast<float4*>(cs + j) = *reinterpret_cast<const float4*>(p.cos + at + j);
-        *reinterpret_cast<float4*>(sn + j) = *reinterpret_cast<const float4*>(p.sin + at + j);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = first ? v[j] * cs[j] - partner[j] * sn[j] : v[j] * cs[j] + partner[j] * sn[j];
-    }
-  }
-  float mn = v[0], mx = v[0], bad = v[0] - v[0];  // bad: 0, or NaN once an element is not finite
-#pragma unroll
-  for (int j = 1; j < 8; ++j) {
-    mn = fminf(mn, v[j]);
-    mx = fmaxf(mx, v[j]);
-    bad += v[j] - v[j];
-  }
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    bad += __shfl_xor_sync(0xffffffffu, bad, o);
-  }
-  const int slot = live ? p.slots[t] : -1;
-  if (live && !is_q && BRAID_IN_BOUNDS(slot >= 0 && slot < p.num_slots, 1, slot) && slot >= 0 && slot < p.num_slots) {
-    // mx - mn passes the fp32 range only for values of magnitude above 1.7e38; such a group counts as not finite
-    const float range = mx - mn;
-    const bool fine = bad == 0.f && range <= 3.4e38f;
-    const __nv_bfloat16 sb = f2bf(fine ? __fdiv_rn(range, 15.f) : __int_as_float(0x7fc00000));
-    const __nv_bfloat16 zb = f2bf(fine ? mn : __int_as_float(0x7fc00000));
-    const float s = bf2f(sb), z = bf2f(zb);
-    uint32_t word = 0;
-    if (fine && s > 0.f) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(v[j] - z, s)), 0.f), 15.f);
-        word |= (uint32_t)c << (4 * j);
+  for (int u = 0; u < U; ++u) {
+    const unsigned item = first + u * IPB;
+    const bool live = item < p.items;
+    tok[u] = live ? item / p.heads : 0u;
+    head[u] = live ? (int)(item - tok[u] * p.heads) + (p.Hq + 2 * p.Hkv - (int)p.heads) : -1;  // within the QKV row
+    raw[u] = make_uint4(0, 0, 0, 0);
+    slot[u] = -1;
+    pos[u] = 0;
+    if (live) {
+      raw[u] = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)tok[u] * p.ld + (int64_t)head[u] * D + l * 8);
+      if (head[u] >= p.Hq) {
+        slot[u] = p.slots[tok[u]];
+        if (p.use_rope) pos[u] = p.positions[tok[u]];
       }
     }
-    const int page = slot / p.PS, off = slot % p.PS;
-    const int kh = is_k ? head - p.Hq : head - p.Hq - p.Hkv;
-    const int64_t row = (((int64_t)page * 2 + (is_k ? 0 : 1)) * p.Hkv + kh) * p.PS + off;
-    p.codes[row * (D / 8) + kv4_word<D>(l)] = word;
-    if (l % 8 == 0)
-      p.scales[row * (D / KV4_GROUP) + l / 8] =
-          (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool live = head[u] >= 0, is_q = live && head[u] < p.Hq, is_k = head[u] >= p.Hq && head[u] < p.Hq + p.Hkv;
+    float v[8];
+    unpack8(raw[u], v);
+    const __nv_bfloat16* nw = is_q ? p.qn : (is_k ? p.kn : nullptr);
+    if (p.kn != nullptr || p.qn != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (nw != nullptr) {
+        const float rstd = rsqrtf(ss / D + p.eps);
+        float wt[8];
+        unpack8(*reinterpret_cast<const uint4*>(nw + l * 8), wt);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * wt[j];
+      }
+    }
+    if (is_q) *reinterpret_cast<uint4*>(p.q_out + ((int64_t)tok[u] * p.Hq + head[u]) * D + l * 8) = pack8(v);
+    if (p.use_rope) {
+      float partner[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) partner[j] = __shfl_xor_sync(0xffffffffu, v[j], LPH / 2);
+      if (is_k) {
+        (void)BRAID_IN_BOUNDS(pos[u] >= 0 && pos[u] < p.rope_len, 2, pos[u]);
+        const int64_t at = (int64_t)min(max(pos[u], 0), p.rope_len - 1) * (D / 2) + (l % (LPH / 2)) * 8;
+        const float sign = l < LPH / 2 ? -1.f : 1.f;
+        float cs[8], sn[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<float4*>(cs + j) = *reinterpret_cast<const float4*>(p.cos + at + j);
+          *reinterpret_cast<float4*>(sn + j) = *reinterpret_cast<const float4*>(p.sin + at + j);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * cs[j] + sign * (partner[j] * sn[j]);
+      }
+    }
+    float mn = v[0], mx = v[0], bad = v[0] - v[0];  // bad: 0, or NaN once an element is not finite
+#pragma unroll
+    for (int j = 1; j < 8; ++j) {
+      mn = fminf(mn, v[j]);
+      mx = fmaxf(mx, v[j]);
+      bad += v[j] - v[j];
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      bad += __shfl_xor_sync(0xffffffffu, bad, o);
+    }
+    if (live && !is_q && BRAID_IN_BOUNDS(slot[u] >= 0 && slot[u] < p.num_slots, 1, slot[u]) && slot[u] >= 0 &&
+        slot[u] < p.num_slots) {
+      // mx - mn passes the fp32 range only for values of magnitude above 1.7e38; such a group counts as not finite
+      const float range = mx - mn;
+      const bool fine = bad == 0.f && range <= 3.4e38f;
+      const __nv_bfloat16 sb = f2bf(fine ? __fdiv_rn(range, 15.f) : __int_as_float(0x7fc00000));
+      const __nv_bfloat16 zb = f2bf(fine ? mn : __int_as_float(0x7fc00000));
+      const float s = bf2f(sb), z = bf2f(zb);
+      uint32_t word = 0;
+      if (fine && s > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float c = fminf(fmaxf(rintf(__fdiv_rn(v[j] - z, s)), 0.f), 15.f);
+          word |= (uint32_t)c << (4 * j);
+        }
+      }
+      const int page = slot[u] / p.PS, off = slot[u] % p.PS;
+      const int kvh = head[u] - p.Hq;  // K heads, then V heads: the cache's order
+      const int64_t row = ((int64_t)page * 2 * p.Hkv + kvh) * p.PS + off;
+      p.codes[row * (D / 8) + kv4_word<D>(l)] = word;
+      if (l % 8 == 0)
+        p.scales[row * (D / KV4_GROUP) + l / 8] =
+            (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+    }
   }
   if (threadIdx.x == 0) span_end(p.span);
 }
 
-// Values 8 l .. 8 l + 7 of a cache row as bf16.
-template <int D>
-BRAID_DEVICE uint4 kv4_values(const uint32_t* codes, const uint32_t* scales, int64_t row, int l) {
-  const uint32_t w = codes[row * (D / 8) + kv4_word<D>(l)];
-  const uint32_t sz = scales[row * (D / KV4_GROUP) + l / 8];
+// Values 8 l .. 8 l + 7 of a cache row from its code word and group pair, as bf16.
+BRAID_DEVICE uint4 kv4_values(uint32_t w, uint32_t sz) {
   const float s = kv4_scale(sz), z = kv4_offset(sz);
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = fmaf(s, (float)((w >> (4 * j)) & 15u), z);
-  return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  return pack8(v);
 }
 
 // out[t, kv, head, :] = the values held at slots[t]; zeros for a slot outside the cache.
-template <int D>
+template <int D, int U>
 __global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* out, const uint32_t* codes,
-                                                       const uint32_t* scales, const int* slots, int64_t items, int Hkv, int PS,
-                                                       int num_slots) {
-  constexpr int LPH = D / 8;
+                                                       const uint32_t* scales, const int* slots, unsigned items,
+                                                       unsigned heads, int PS, int num_slots) {
+  constexpr int LPH = D / 8, IPB = 256 / LPH;
   pdl_trigger();
   pdl_wait();
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
   const int l = threadIdx.x % LPH;
-  if (item >= items) return;
-  const int64_t t = item / (2 * Hkv);
-  const int kvh = (int)(item % (2 * Hkv));
-  const int slot = slots[t];
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (BRAID_IN_BOUNDS(slot >= 0 && slot < num_slots, 1, slot) && slot >= 0 && slot < num_slots) {
-    const int64_t row = ((int64_t)(slot / PS) * 2 * Hkv + kvh) * PS + slot % PS;
-    o = kv4_values<D>(codes, scales, row, l);
+  const unsigned first = blockIdx.x * (IPB * U) + threadIdx.x / LPH;
+  uint32_t w[U], sz[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned item = first + u * IPB;
+    w[u] = sz[u] = 0u;  // stands for zeros
+    if (item < items) {
+      const unsigned t = item / heads;
+      const int slot = slots[t];
+      if (BRAID_IN_BOUNDS(slot >= 0 && slot < num_slots, 1, slot) && slot >= 0 && slot < num_slots) {
+        const int64_t row = ((int64_t)(slot / PS) * heads + (item - t * heads)) * PS + slot % PS;
+        w[u] = codes[row * (D / 8) + kv4_word<D>(l)];
+        sz[u] = scales[row * (D / KV4_GROUP) + l / 8];
+      }
+    }
   }
-  *reinterpret_cast<uint4*>(out + item * D + l * 8) = o;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned item = first + u * IPB;
+    if (item < items) *reinterpret_cast<uint4*>(out + (int64_t)item * D + l * 8) = kv4_values(w[u], sz[u]);
+  }
 }
 
 // Page i of the plan's list as bf16 page i of `out` [NP, 2, Hkv, PS, D], for the long-prompt attention: the slots of its
@@ -228,7 +257,7 @@ __global__ void __launch_bounds__(256) kv4_unpack_pages_kernel(__nv_bfloat16* ou
   for (int e = threadIdx.x; e < p.PS * LPR; e += 256) {
     const int r = e / LPR, l = e % LPR;
     uint4 o = make_uint4(0, 0, 0, 0);
-    if (slot0 + r - off >= a && slot0 + r - off < b) o = kv4_values<D>(codes, p.scales, src + r, l);
+    if (slot0 + r - off >= a && slot0 + r - off < b) o = kv4_values(codes[(src + r) * (D / 8) + kv4_word<D>(l)], p.scales[(src + r) * (D / KV4_GROUP) + l / 8]);
     *reinterpret_cast<uint4*>(out + (dst + r) * D + l * 8) = o;
   }
 }
@@ -283,8 +312,9 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
   const bool has_qn = q_norm.has_value() && q_norm->defined(), has_kn = k_norm.has_value() && k_norm->defined();
   for (const auto* w : {has_qn ? &*q_norm : nullptr, has_kn ? &*k_norm : nullptr})
     if (w != nullptr)
-      TORCH_CHECK(w->device() == dev && w->scalar_type() == at::kBFloat16 && w->numel() == D && w->is_contiguous(), who,
-                  ": norm weights must be contiguous bf16 [D] on the device of the cache");
+      TORCH_CHECK(w->device() == dev && w->scalar_type() == at::kBFloat16 && w->numel() == D && w->is_contiguous() &&
+                      reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0,
+                  who, ": norm weights must be contiguous, 16-byte aligned bf16 [D] on the device of the cache");
   if (use_rope)
     TORCH_CHECK(cos.device() == dev && sin.device() == dev && cos.scalar_type() == at::kFloat &&
                     sin.scalar_type() == at::kFloat && cos.is_contiguous() && sin.is_contiguous() && cos.dim() == 2 &&
@@ -308,8 +338,9 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
   p.sin = use_rope ? sin.data_ptr<float>() : nullptr;
   p.eps = (float)eps;
   p.ld = qkv.stride(0);
-  p.heads = (int)(2 * Hkv + (has_qn ? Hq : 0));
-  p.items = T * p.heads;
+  p.heads = (unsigned)(2 * Hkv + (has_qn ? Hq : 0));
+  TORCH_CHECK(T * p.heads < (1ll << 31), who, ": more than 2^31 (token, head) rows");
+  p.items = (unsigned)(T * p.heads);
   p.Hq = (int)Hq;
   p.Hkv = (int)Hkv;
   p.PS = (int)codes.size(3);
@@ -317,13 +348,17 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
   p.num_slots = (int)(codes.size(0) * codes.size(3));
   p.rope_len = use_rope ? (int)cos.size(0) : 1;
   p.span = next_span("qkv_prepare_kv4");
-  const int64_t per_block = 256 / (D / 8);
-  const dim3 grid((unsigned)((p.items + per_block - 1) / per_block));
   auto st = at::cuda::getCurrentCUDAStream();
+  const auto go = [&](auto k, unsigned per_block) {
+    launch_pdl(k, dim3((p.items + per_block - 1) / per_block), dim3(256), 0, st, p);
+  };
+  // several items a thread once one each fills the SMs' resident blocks (8 of 256 threads) twice
+  const unsigned ipb = (unsigned)(256 / (D / 8));
+  const bool many = p.items >= ipb * 16 * (unsigned)gemm_num_sms();
   if (D == 128)
-    launch_pdl(qkv_prepare_kv4_kernel<128>, grid, dim3(256), 0, st, p);
+    many ? go(qkv_prepare_kv4_kernel<128, 4>, 4 * ipb) : go(qkv_prepare_kv4_kernel<128, 1>, ipb);
   else
-    launch_pdl(qkv_prepare_kv4_kernel<64>, grid, dim3(256), 0, st, p);
+    many ? go(qkv_prepare_kv4_kernel<64, 4>, 4 * ipb) : go(qkv_prepare_kv4_kernel<64, 1>, ipb);
 }
 
 void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torch::Tensor slots) {
@@ -335,19 +370,21 @@ void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torc
   TORCH_CHECK(out.device() == codes.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
                   out.numel() == T * 2 * Hkv * D,
               who, ": out must be a contiguous bf16 [T, 2, Hkv, D] tensor");
+  TORCH_CHECK(T * 2 * Hkv < (1ll << 31), who, ": more than 2^31 (slot, head) rows");
   const at::cuda::CUDAGuard g(codes.device());
-  const int64_t items = T * 2 * Hkv, per_block = 256 / (D / 8);
-  const dim3 grid((unsigned)((items + per_block - 1) / per_block));
+  const unsigned items = (unsigned)(T * 2 * Hkv), ipb = (unsigned)(256 / (D / 8));
   auto st = at::cuda::getCurrentCUDAStream();
-  auto* o = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
-  const auto* c = reinterpret_cast<const uint32_t*>(codes.data_ptr());
-  const auto* s = reinterpret_cast<const uint32_t*>(scales.data_ptr());
+  const auto go = [&](auto k, unsigned per_block) {
+    launch_pdl(k, dim3((items + per_block - 1) / per_block), dim3(256), 0, st,
+               reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), reinterpret_cast<const uint32_t*>(codes.data_ptr()),
+               reinterpret_cast<const uint32_t*>(scales.data_ptr()), (const int*)slots.data_ptr<int>(), items,
+               (unsigned)(2 * Hkv), (int)PS, (int)(codes.size(0) * PS));
+  };
+  const bool many = items >= ipb * 16 * (unsigned)gemm_num_sms();
   if (D == 128)
-    launch_pdl(kv4_read_kernel<128>, grid, dim3(256), 0, st, o, c, s, (const int*)slots.data_ptr<int>(), items, (int)Hkv,
-               (int)PS, (int)(codes.size(0) * PS));
+    many ? go(kv4_read_kernel<128, 4>, 4 * ipb) : go(kv4_read_kernel<128, 1>, ipb);
   else
-    launch_pdl(kv4_read_kernel<64>, grid, dim3(256), 0, st, o, c, s, (const int*)slots.data_ptr<int>(), items, (int)Hkv,
-               (int)PS, (int)(codes.size(0) * PS));
+    many ? go(kv4_read_kernel<64, 4>, 4 * ipb) : go(kv4_read_kernel<64, 1>, ipb);
 }
 
 BRAID_BOUNDS_READER(bounds_status_kv4)
