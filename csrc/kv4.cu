@@ -18,6 +18,18 @@ namespace braid {
 unsigned long long* next_span(const char* name);
 int gemm_num_sms();
 
+// n / d of 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + k) / d) with 2^k >= d.
+struct FastDiv {
+  unsigned d, m, shift;
+  explicit FastDiv(unsigned div = 1) : d(div), m(0), shift(0) {
+    unsigned k = 0;
+    while ((1ull << k) < div) ++k;
+    m = (unsigned)(((1ull << (31 + k)) + div - 1) / div);
+    shift = k;
+  }
+  BRAID_DEVICE unsigned div(unsigned n) const { return (unsigned)(((uint64_t)n * m) >> 31) >> shift; }
+};
+
 struct Kv4AppendParams {
   const __nv_bfloat16* qkv;  // [T, ld] rows of (Hq + 2 Hkv) heads
   __nv_bfloat16* q_out;      // [T, Hq, D], written only with a q norm
@@ -32,8 +44,9 @@ struct Kv4AppendParams {
   float eps;
   int64_t ld;
   unsigned items;            // T * heads handled
-  unsigned heads;            // handled per token: 2 Hkv, or Hq + 2 Hkv with a q norm
-  int Hq, Hkv, PS, use_rope, num_slots, rope_len;
+  FastDiv heads;             // handled per token: 2 Hkv, or Hq + 2 Hkv with a q norm
+  FastDiv page;              // slots of a page
+  int Hq, Hkv, use_rope, num_slots, rope_len;
   unsigned long long* span;
 };
 
@@ -47,6 +60,28 @@ BRAID_DEVICE void unpack8(uint4 u, float* v) {
 }
 BRAID_DEVICE uint4 pack8(const float* v) {
   return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// Eight codes round((v - z) / s), ties to even, clamped to 0..15.  bf16 inputs
+// put many quotients exactly on a tie, so a product with 1 / s alone would often
+// fall to the wrong side.  It gives a candidate c within one of the answer; its
+// residual d - c s (c s has 12 bits and is exact) then decides as the exact
+// quotient would: beyond half a step, or on it with c odd, c moves by one.
+BRAID_DEVICE uint32_t kv4_codes(const float* v, float s, float z) {
+  const float r = __fdividef(1.f, s);
+  float c[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float d = v[j] - z;
+    const float t = fmaf(d, r, 12582912.f);  // the integer lands in the low bits of the sum
+    c[j] = t - 12582912.f;
+    const float e = fmaf(-c[j], s, d), h = fabsf(e + e);
+    if (h > s || (h == s && (__float_as_uint(t) & 1u))) c[j] += e > 0.f ? 1.f : -1.f;
+    c[j] = fminf(fmaxf(c[j], 0.f), 15.f);
+  }
+  const float lo = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]);
+  const float hi = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]);
+  return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
 // D / 8 lanes per (token, head), 8 elements (one 16-byte load, one code word)
@@ -70,8 +105,8 @@ __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendPar
   for (int u = 0; u < U; ++u) {
     const unsigned item = first + u * IPB;
     const bool live = item < p.items;
-    tok[u] = live ? item / p.heads : 0u;
-    head[u] = live ? (int)(item - tok[u] * p.heads) + (p.Hq + 2 * p.Hkv - (int)p.heads) : -1;  // within the QKV row
+    tok[u] = live ? p.heads.div(item) : 0u;
+    head[u] = live ? (int)(item - tok[u] * p.heads.d) + (p.Hq + 2 * p.Hkv - (int)p.heads.d) : -1;  // within the QKV row
     raw[u] = make_uint4(0, 0, 0, 0);
     slot[u] = -1;
     pos[u] = 0;
@@ -89,7 +124,7 @@ __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendPar
     float v[8];
     unpack8(raw[u], v);
     const __nv_bfloat16* nw = is_q ? p.qn : (is_k ? p.kn : nullptr);
-    if (p.kn != nullptr || p.qn != nullptr) {
+    if (__any_sync(0xffffffffu, nw != nullptr)) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
@@ -104,7 +139,8 @@ __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendPar
       }
     }
     if (is_q) *reinterpret_cast<uint4*>(p.q_out + ((int64_t)tok[u] * p.Hq + head[u]) * D + l * 8) = pack8(v);
-    if (p.use_rope) {
+    if (__all_sync(0xffffffffu, head[u] < p.Hq)) continue;  // nothing of this warp goes into the cache
+    if (p.use_rope && __any_sync(0xffffffffu, is_k)) {
       float partner[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) partner[j] = __shfl_xor_sync(0xffffffffu, v[j], LPH / 2);
@@ -122,38 +158,32 @@ __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendPar
         for (int j = 0; j < 8; ++j) v[j] = v[j] * cs[j] + sign * (partner[j] * sn[j]);
       }
     }
-    float mn = v[0], mx = v[0], bad = v[0] - v[0];  // bad: 0, or NaN once an element is not finite
+    float mn = v[0], mx = v[0], bad = v[0] * 0.f;  // bad: 0, or NaN once an element is not finite
 #pragma unroll
     for (int j = 1; j < 8; ++j) {
       mn = fminf(mn, v[j]);
       mx = fmaxf(mx, v[j]);
-      bad += v[j] - v[j];
+      bad = fmaf(v[j], 0.f, bad);
     }
+    if (bad != 0.f) mx = INFINITY;  // the group's range is then infinite
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) {
       mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      bad += __shfl_xor_sync(0xffffffffu, bad, o);
     }
     if (live && !is_q && BRAID_IN_BOUNDS(slot[u] >= 0 && slot[u] < p.num_slots, 1, slot[u]) && slot[u] >= 0 &&
         slot[u] < p.num_slots) {
       // mx - mn passes the fp32 range only for values of magnitude above 1.7e38; such a group counts as not finite
       const float range = mx - mn;
-      const bool fine = bad == 0.f && range <= 3.4e38f;
+      const bool fine = range <= 3.4e38f;
       const __nv_bfloat16 sb = f2bf(fine ? __fdiv_rn(range, 15.f) : __int_as_float(0x7fc00000));
       const __nv_bfloat16 zb = f2bf(fine ? mn : __int_as_float(0x7fc00000));
       const float s = bf2f(sb), z = bf2f(zb);
       uint32_t word = 0;
-      if (fine && s > 0.f) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float c = fminf(fmaxf(rintf(__fdiv_rn(v[j] - z, s)), 0.f), 15.f);
-          word |= (uint32_t)c << (4 * j);
-        }
-      }
-      const int page = slot[u] / p.PS, off = slot[u] % p.PS;
+      if (fine && s > 0.f) word = kv4_codes(v, s, z);
+      const unsigned page = p.page.div((unsigned)slot[u]), off = (unsigned)slot[u] - page * p.page.d;
       const int kvh = head[u] - p.Hq;  // K heads, then V heads: the cache's order
-      const int64_t row = ((int64_t)page * 2 * p.Hkv + kvh) * p.PS + off;
+      const int64_t row = (int64_t)(page * 2 * p.Hkv + kvh) * p.page.d + off;  // page * heads: below 2^31 rows
       p.codes[row * (D / 8) + kv4_word<D>(l)] = word;
       if (l % 8 == 0)
         p.scales[row * (D / KV4_GROUP) + l / 8] =
@@ -168,7 +198,8 @@ BRAID_DEVICE uint4 kv4_values(uint32_t w, uint32_t sz) {
   const float s = kv4_scale(sz), z = kv4_offset(sz);
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = fmaf(s, (float)((w >> (4 * j)) & 15u), z);
+  for (int j = 0; j < 8; ++j)  // 2^23 + c by its bits, then c exactly (a conversion would take the slow unit)
+    v[j] = fmaf(s, __uint_as_float(((w >> (4 * j)) & 15u) | 0x4B000000u) - 8388608.f, z);
   return pack8(v);
 }
 
@@ -176,7 +207,8 @@ BRAID_DEVICE uint4 kv4_values(uint32_t w, uint32_t sz) {
 template <int D, int U>
 __global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* out, const uint32_t* codes,
                                                        const uint32_t* scales, const int* slots, unsigned items,
-                                                       unsigned heads, int PS, int num_slots) {
+                                                       FastDiv heads, FastDiv page_div,
+                                                       int num_slots) {
   constexpr int LPH = D / 8, IPB = 256 / LPH;
   pdl_trigger();
   pdl_wait();
@@ -188,10 +220,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(__nv_bfloat16* out, const
     const unsigned item = first + u * IPB;
     w[u] = sz[u] = 0u;  // stands for zeros
     if (item < items) {
-      const unsigned t = item / heads;
+      const unsigned t = heads.div(item);
       const int slot = slots[t];
       if (BRAID_IN_BOUNDS(slot >= 0 && slot < num_slots, 1, slot) && slot >= 0 && slot < num_slots) {
-        const int64_t row = ((int64_t)(slot / PS) * heads + (item - t * heads)) * PS + slot % PS;
+        const unsigned page = page_div.div((unsigned)slot), off = (unsigned)slot - page * page_div.d;
+        const int64_t row = (int64_t)(page * heads.d + (item - t * heads.d)) * page_div.d + off;
         w[u] = codes[row * (D / 8) + kv4_word<D>(l)];
         sz[u] = scales[row * (D / KV4_GROUP) + l / 8];
       }
@@ -282,7 +315,9 @@ void kv4_check_layer(const torch::Tensor& codes, const torch::Tensor& scales, co
                   scales.size(2) == codes.size(2) && scales.size(3) == codes.size(3) &&
                   scales.size(4) == D / KV4_GROUP && scales.size(5) == 2,
               who, ": 4-bit cache codes and scales do not match");
-  TORCH_CHECK(codes.size(0) * codes.size(3) < (1ll << 31), who, ": more than 2^31 slots");
+  TORCH_CHECK(codes.size(3) > 0 && codes.size(0) * codes.size(3) < (1ll << 31) &&
+                  codes.size(0) * 2 * codes.size(2) < (1ll << 31),
+              who, ": more than 2^31 slots or (page, head) slabs");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
               who, ": 4-bit cache tensors must be 16-byte aligned");
@@ -338,12 +373,12 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
   p.sin = use_rope ? sin.data_ptr<float>() : nullptr;
   p.eps = (float)eps;
   p.ld = qkv.stride(0);
-  p.heads = (unsigned)(2 * Hkv + (has_qn ? Hq : 0));
-  TORCH_CHECK(T * p.heads < (1ll << 31), who, ": more than 2^31 (token, head) rows");
-  p.items = (unsigned)(T * p.heads);
+  p.heads = FastDiv((unsigned)(2 * Hkv + (has_qn ? Hq : 0)));
+  p.page = FastDiv((unsigned)codes.size(3));
+  TORCH_CHECK(T * p.heads.d < (1ll << 31), who, ": more than 2^31 (token, head) rows");
+  p.items = (unsigned)(T * p.heads.d);
   p.Hq = (int)Hq;
   p.Hkv = (int)Hkv;
-  p.PS = (int)codes.size(3);
   p.use_rope = use_rope ? 1 : 0;
   p.num_slots = (int)(codes.size(0) * codes.size(3));
   p.rope_len = use_rope ? (int)cos.size(0) : 1;
@@ -378,7 +413,7 @@ void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torc
     launch_pdl(k, dim3((items + per_block - 1) / per_block), dim3(256), 0, st,
                reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), reinterpret_cast<const uint32_t*>(codes.data_ptr()),
                reinterpret_cast<const uint32_t*>(scales.data_ptr()), (const int*)slots.data_ptr<int>(), items,
-               (unsigned)(2 * Hkv), (int)PS, (int)(codes.size(0) * PS));
+               FastDiv((unsigned)(2 * Hkv)), FastDiv((unsigned)PS), (int)(codes.size(0) * PS));
   };
   const bool many = items >= ipb * 16 * (unsigned)gemm_num_sms();
   if (D == 128)
