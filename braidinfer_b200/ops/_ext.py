@@ -33,15 +33,16 @@ class _Counted:
 
     def __getattr__(self, name):
         fn = getattr(self._mod, name)
-        if not callable(fn) or name in _NOT_LAUNCHES:
-            return fn
+        if callable(fn) and name not in _NOT_LAUNCHES:
+            native = fn
 
-        def call(*a, **kw):
-            global launches
-            launches += 1
-            return fn(*a, **kw)
+            def fn(*a, **kw):
+                global launches
+                launches += 1
+                return native(*a, **kw)
 
-        return call
+        self.__dict__[name] = fn  # later calls find it without this function
+        return fn
 
 
 def count(n: int) -> None:

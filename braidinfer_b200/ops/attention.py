@@ -117,15 +117,12 @@ def qkv_prepare(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.
 
 def _qkv_prepare_kv4(qkv, positions, slot_mapping, kv_layer, num_q_heads, num_kv_heads, head_dim, cos, sin, q_norm,
                      k_norm, eps, use_rope):
-    T = qkv.shape[0]
     codes, scales = kv_layer
+    if qkv.is_cuda:
+        return ext().qkv_prepare_kv4(qkv, positions, slot_mapping, codes, scales, q_norm, k_norm, float(eps), cos, sin,
+                                     num_q_heads, num_kv_heads, head_dim, bool(use_rope))
     qs = num_q_heads * head_dim
     view = qkv[:, :qs].unflatten(1, (num_q_heads, head_dim))
-    if qkv.is_cuda:
-        q = view if q_norm is None else torch.empty(T, num_q_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
-        ext().qkv_prepare_kv4(q, qkv, positions, slot_mapping, codes, scales, q_norm, k_norm, float(eps), cos, sin,
-                              num_q_heads, num_kv_heads, head_dim, bool(use_rope))
-        return q
 
     def norm(x, w):
         return x if w is None else x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w.float()
@@ -250,15 +247,14 @@ def attention(q: torch.Tensor, kv_layer: Union[torch.Tensor, KV4Layer], meta: At
     if (q4 or window > 0) and meta.seq_nsh is not None:
         raise ValueError("attention: a shared-prefix plan takes neither a 4-bit cache nor a window")
     if q.is_cuda:
-        T, Hq, D = q.shape
-        out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
         if q4 or window > 0:
             kv, scales = kv_layer if q4 else (kv_layer, None)
-            ext().attention_rows(out, q, kv, scales, meta.qo_indptr, meta.positions, meta.seg_indptr,
-                                 meta.seg_page_indptr, meta.seg_offset, meta.seg_len, meta.seg_pos0, meta.seg_delta,
-                                 meta.page_ids, cos, sin, float(scale), bool(use_rope), int(meta.num_seqs),
-                                 int(meta.max_q_len), int(meta.max_kv_len), window, sinks)
-            return out
+            return ext().attention_rows(None, q, kv, scales, meta.qo_indptr, meta.positions, meta.seg_indptr,
+                                        meta.seg_page_indptr, meta.seg_offset, meta.seg_len, meta.seg_pos0,
+                                        meta.seg_delta, meta.page_ids, cos, sin, float(scale), bool(use_rope),
+                                        int(meta.num_seqs), int(meta.max_q_len), int(meta.max_kv_len), window, sinks)
+        T, Hq, D = q.shape
+        out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
         ws = workspace or {}
         ext().attention(out, q, kv_layer, meta.qo_indptr, meta.positions, meta.seg_indptr,
                         meta.seg_page_indptr, meta.seg_offset, meta.seg_len, meta.seg_pos0, meta.seg_delta,

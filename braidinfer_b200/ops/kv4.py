@@ -103,14 +103,11 @@ def kv4_read(kv_layer: KV4Layer, slots: torch.Tensor) -> torch.Tensor:
     ``page * page_size + offset``) as ``[T, 2, Hkv, D]`` bf16, rounded once;
     zeros for a slot outside the cache."""
     codes, scales = kv_layer
-    P, _, Hkv, ps, half = codes.shape
     if slots.dim() != 1:
         raise ValueError("kv4_read: slots must be one-dimensional")
     if codes.is_cuda:
-        out = torch.empty(slots.shape[0], 2, Hkv, half * 2, dtype=torch.bfloat16, device=codes.device)
-        ext().kv4_read(out, codes, scales, slots)
-        return out
-    s = slots.long()
+        return ext().kv4_read(codes, scales, slots)
+    P, ps, s = codes.shape[0], codes.shape[3], slots.long()
     ok = (s >= 0) & (s < P * ps)
     s = torch.where(ok, s, torch.zeros_like(s))
     v = kv4_unpack_ref(codes[s // ps, :, :, s % ps], scales[s // ps, :, :, s % ps])

@@ -1176,12 +1176,13 @@ static void attention_prompt(const RowsParams& r, const torch::Tensor* pool, con
 }
 
 // Attention of few rows over a bf16 layer pool (`kv`, `scales` undefined) or a
-// 4-bit layer (`kv` = codes), with an optional window.
-void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::optional<torch::Tensor> scales,
-                    torch::Tensor qo_indptr, torch::Tensor positions, torch::Tensor seg_indptr,
-                    torch::Tensor seg_page_indptr, torch::Tensor seg_offset, torch::Tensor seg_len,
-                    torch::Tensor seg_pos0, torch::Tensor seg_delta, torch::Tensor page_ids, torch::Tensor cos,
-                    torch::Tensor sin, double scale, bool use_rope, int64_t num_seqs, int64_t max_q_len,
+// 4-bit layer (`kv` = codes), with an optional window; into `out` if given.
+torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const torch::Tensor& q, const torch::Tensor& kv,
+                    const c10::optional<torch::Tensor>& scales, const torch::Tensor& qo_indptr,
+                    const torch::Tensor& positions, const torch::Tensor& seg_indptr,
+                    const torch::Tensor& seg_page_indptr, const torch::Tensor& seg_offset, const torch::Tensor& seg_len,
+                    const torch::Tensor& seg_pos0, const torch::Tensor& seg_delta, const torch::Tensor& page_ids,
+                    const torch::Tensor& cos, const torch::Tensor& sin, double scale, bool use_rope, int64_t num_seqs, int64_t max_q_len,
                     int64_t max_kv_len, int64_t window, int64_t sinks) {
   const bool q4 = scales.has_value() && scales->defined();
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3, "attention: q must be bf16 [T, Hq, D]");
@@ -1198,6 +1199,9 @@ void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::o
                     kv.size(1) == 2 && reinterpret_cast<uintptr_t>(kv.data_ptr()) % 16 == 0,
                 "attention: cache must be a contiguous bf16 tensor [P, 2, Hkv, page, D]");
   }
+  const at::cuda::CUDAGuard guard(dev);
+  const bool given = out_arg.has_value() && out_arg->defined();
+  const torch::Tensor out = given ? *out_arg : at::empty({T, Hq * D}, q.options());
   TORCH_CHECK(kv.device() == dev && out.device() == dev, "attention: q, cache and out on different devices");
   const int64_t Hkv = kv.size(2), PS = kv.size(3);
   TORCH_CHECK(kv.size(4) == (q4 ? D / 2 : D) && Hkv > 0 && Hq % Hkv == 0, "attention: head layout mismatch");
@@ -1207,7 +1211,7 @@ void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::o
   TORCH_CHECK(window >= 0 && window < (1ll << 30) && sinks >= 0 && sinks < (1ll << 30),
               "attention: window and sinks must be in [0, 2^30)");
   TORCH_CHECK(num_seqs >= 0 && max_q_len >= 0 && max_q_len <= T, "attention: max_q_len must be in [0, T]");
-  if (T == 0 || num_seqs == 0 || max_q_len == 0) return;
+  if (T == 0 || num_seqs == 0 || max_q_len == 0) return out;
   const auto i32 = [&](const torch::Tensor& t, int64_t n, const char* name) {
     TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == dev && t.numel() >= n, "attention: ",
                 name, " must be a contiguous int32 tensor of at least ", std::to_string(n), " elements on the device of the cache");
@@ -1248,7 +1252,6 @@ void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::o
   p.num_pages = (int)kv.size(0);
   p.window = (int)window;
   p.sinks = (int)sinks;
-  const at::cuda::CUDAGuard guard(dev);
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   p.span = next_span("attn_rows");
   int64_t keys = std::max<int64_t>(1, max_kv_len);
@@ -1256,7 +1259,7 @@ void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::o
   const int64_t rows = max_q_len * p.G;
   if (max_q_len > 1 && attn_prefill_tc_use((int)D, T * p.G)) {
     attention_prompt(p, q4 ? nullptr : &kv, kv, scales, T, num_seqs, max_q_len, keys, page_ids.numel(), st);
-    return;
+    return out;
   }
   const auto pick = [&](auto d, auto bits) {
     constexpr int DD = decltype(d)::value, BB = decltype(bits)::value;
@@ -1276,6 +1279,7 @@ void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::o
     pick(integral_constant<int, 64>{}, integral_constant<int, 4>{});
   else
     pick(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+  return out;
 }
 
 BRAID_BOUNDS_READER(bounds_status_attention_rows)

@@ -73,17 +73,20 @@ void attention(torch::Tensor out, torch::Tensor q, torch::Tensor kv, torch::Tens
                c10::optional<torch::Tensor> part_o, c10::optional<torch::Tensor> part_lse,
                c10::optional<torch::Tensor> grp_qo_indptr, c10::optional<torch::Tensor> grp_seg_indptr,
                c10::optional<torch::Tensor> seq_nsh, int64_t shared_splits, int64_t grp_max_q);
-void attention_rows(torch::Tensor out, torch::Tensor q, torch::Tensor kv, c10::optional<torch::Tensor> scales,
-                    torch::Tensor qo_indptr, torch::Tensor positions, torch::Tensor seg_indptr,
-                    torch::Tensor seg_page_indptr, torch::Tensor seg_offset, torch::Tensor seg_len,
-                    torch::Tensor seg_pos0, torch::Tensor seg_delta, torch::Tensor page_ids, torch::Tensor cos,
-                    torch::Tensor sin, double scale, bool use_rope, int64_t num_seqs, int64_t max_q_len,
-                    int64_t max_kv_len, int64_t window, int64_t sinks);
-void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor slots,
-                     torch::Tensor codes, torch::Tensor scales, c10::optional<torch::Tensor> q_norm,
-                     c10::optional<torch::Tensor> k_norm, double eps, torch::Tensor cos, torch::Tensor sin,
-                     int64_t Hq, int64_t Hkv, int64_t D, bool use_rope);
-void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torch::Tensor slots);
+torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out, const torch::Tensor& q, const torch::Tensor& kv,
+                             const c10::optional<torch::Tensor>& scales, const torch::Tensor& qo_indptr,
+                             const torch::Tensor& positions, const torch::Tensor& seg_indptr,
+                             const torch::Tensor& seg_page_indptr, const torch::Tensor& seg_offset,
+                             const torch::Tensor& seg_len, const torch::Tensor& seg_pos0,
+                             const torch::Tensor& seg_delta, const torch::Tensor& page_ids, const torch::Tensor& cos,
+                             const torch::Tensor& sin, double scale, bool use_rope, int64_t num_seqs,
+                             int64_t max_q_len, int64_t max_kv_len, int64_t window, int64_t sinks);
+torch::Tensor qkv_prepare_kv4(const torch::Tensor& qkv, const torch::Tensor& positions, const torch::Tensor& slots,
+                              const torch::Tensor& codes, const torch::Tensor& scales,
+                              const c10::optional<torch::Tensor>& q_norm, const c10::optional<torch::Tensor>& k_norm,
+                              double eps, const torch::Tensor& cos, const torch::Tensor& sin, int64_t Hq, int64_t Hkv,
+                              int64_t D, bool use_rope);
+torch::Tensor kv4_read(const torch::Tensor& codes, const torch::Tensor& scales, const torch::Tensor& slots);
 void attn_set_trace(torch::Tensor buf);
 void attn_tc_set_trace(torch::Tensor buf);
 void attn_select_prefill_tc(int64_t mode);

@@ -328,10 +328,12 @@ static void check_i32(const torch::Tensor& t, int64_t n, const torch::Device& de
               " must be a contiguous int32 tensor of at least ", std::to_string(n), " elements on the device of the cache");
 }
 
-void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor slots,
-                     torch::Tensor codes, torch::Tensor scales, c10::optional<torch::Tensor> q_norm,
-                     c10::optional<torch::Tensor> k_norm, double eps, torch::Tensor cos, torch::Tensor sin,
-                     int64_t Hq, int64_t Hkv, int64_t D, bool use_rope) {
+// Returns q [T, Hq, D]: the normalised queries, or without a q norm their columns of qkv.
+torch::Tensor qkv_prepare_kv4(const torch::Tensor& qkv, const torch::Tensor& positions, const torch::Tensor& slots,
+                              const torch::Tensor& codes, const torch::Tensor& scales,
+                              const c10::optional<torch::Tensor>& q_norm, const c10::optional<torch::Tensor>& k_norm,
+                              double eps, const torch::Tensor& cos, const torch::Tensor& sin, int64_t Hq, int64_t Hkv,
+                              int64_t D, bool use_rope) {
   const char* who = "qkv_prepare";
   kv4_check_layer(codes, scales, who);
   const auto dev = codes.device();
@@ -341,10 +343,13 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
               who, ": qkv must be a bf16 [T, (Hq + 2 Hkv) D] tensor with 16-byte aligned rows on the device of the cache");
   TORCH_CHECK(codes.size(2) == Hkv && codes.size(4) * 2 == D, who, ": cache layout mismatch");
   const int64_t T = qkv.size(0);
-  if (T == 0) return;
+  const bool has_qn = q_norm.has_value() && q_norm->defined(), has_kn = k_norm.has_value() && k_norm->defined();
+  const at::cuda::CUDAGuard g(dev);
+  const torch::Tensor q_out =
+      has_qn ? at::empty({T, Hq, D}, qkv.options()) : qkv.as_strided({T, Hq, D}, {qkv.stride(0), D, 1});
+  if (T == 0) return q_out;
   check_i32(positions, T, dev, who, "positions");
   check_i32(slots, T, dev, who, "slots");
-  const bool has_qn = q_norm.has_value() && q_norm->defined(), has_kn = k_norm.has_value() && k_norm->defined();
   for (const auto* w : {has_qn ? &*q_norm : nullptr, has_kn ? &*k_norm : nullptr})
     if (w != nullptr)
       TORCH_CHECK(w->device() == dev && w->scalar_type() == at::kBFloat16 && w->numel() == D && w->is_contiguous() &&
@@ -355,11 +360,6 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
                     sin.scalar_type() == at::kFloat && cos.is_contiguous() && sin.is_contiguous() && cos.dim() == 2 &&
                     cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes(),
                 who, ": cos and sin must be contiguous fp32 [positions, D/2] tables on the device of the cache");
-  if (has_qn)
-    TORCH_CHECK(q_out.device() == dev && q_out.scalar_type() == at::kBFloat16 && q_out.is_contiguous() &&
-                    q_out.numel() == T * Hq * D,
-                who, ": q_out must be a contiguous bf16 [T, Hq, D] tensor");
-  const at::cuda::CUDAGuard g(dev);
   Kv4AppendParams p{};
   p.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
   p.q_out = has_qn ? reinterpret_cast<__nv_bfloat16*>(q_out.data_ptr()) : nullptr;
@@ -394,19 +394,19 @@ void qkv_prepare_kv4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor posit
     many ? go(qkv_prepare_kv4_kernel<128, 4>, 4 * ipb) : go(qkv_prepare_kv4_kernel<128, 1>, ipb);
   else
     many ? go(qkv_prepare_kv4_kernel<64, 4>, 4 * ipb) : go(qkv_prepare_kv4_kernel<64, 1>, ipb);
+  return q_out;
 }
 
-void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torch::Tensor slots) {
+// bf16 [T, 2, Hkv, D] of what the cache holds at `slots`.
+torch::Tensor kv4_read(const torch::Tensor& codes, const torch::Tensor& scales, const torch::Tensor& slots) {
   const char* who = "kv4_read";
   kv4_check_layer(codes, scales, who);
   const int64_t T = slots.numel(), Hkv = codes.size(2), PS = codes.size(3), D = codes.size(4) * 2;
-  if (T == 0) return;
-  check_i32(slots, T, codes.device(), who, "slots");
-  TORCH_CHECK(out.device() == codes.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
-                  out.numel() == T * 2 * Hkv * D,
-              who, ": out must be a contiguous bf16 [T, 2, Hkv, D] tensor");
-  TORCH_CHECK(T * 2 * Hkv < (1ll << 31), who, ": more than 2^31 (slot, head) rows");
   const at::cuda::CUDAGuard g(codes.device());
+  const torch::Tensor out = at::empty({T, 2, Hkv, D}, scales.options());
+  if (T == 0) return out;
+  check_i32(slots, T, codes.device(), who, "slots");
+  TORCH_CHECK(T * 2 * Hkv < (1ll << 31), who, ": more than 2^31 (slot, head) rows");
   const unsigned items = (unsigned)(T * 2 * Hkv), ipb = (unsigned)(256 / (D / 8));
   auto st = at::cuda::getCurrentCUDAStream();
   const auto go = [&](auto k, unsigned per_block) {
@@ -420,6 +420,7 @@ void kv4_read(torch::Tensor out, torch::Tensor codes, torch::Tensor scales, torc
     many ? go(kv4_read_kernel<128, 4>, 4 * ipb) : go(kv4_read_kernel<128, 1>, ipb);
   else
     many ? go(kv4_read_kernel<64, 4>, 4 * ipb) : go(kv4_read_kernel<64, 1>, ipb);
+  return out;
 }
 
 BRAID_BOUNDS_READER(bounds_status_kv4)
