@@ -119,9 +119,11 @@ struct RowsShape {
   static constexpr int D = D_, BITS = BITS_, NT = NT_;
   static constexpr int ROWS = 8 * NT;
   static constexpr bool Q4 = BITS == 4;
-  static constexpr int MB = 1;                        // 16-key MMA tiles of a step
+  // 16-key MMA tiles of a step: two independent ones keep a warp's pipes busier (steady decode from a 4-bit cache 3.94
+  // -> 4.28 TB/s); with more row tiles the registers do not allow it
+  static constexpr int MB = Q4 && NT == 1 ? 2 : 1;
   static constexpr int KB = 16 * MB;                  // keys of a step
-  static constexpr int SUB = (Q4 || D == 64) ? 2 : 1; // steps per consumer and tile
+  static constexpr int SUB = ((Q4 || D == 64) ? 2 : 1) / MB; // steps per consumer and tile
   static constexpr int TILE = ROWS_WARPS * SUB * KB;  // keys per tile
   static constexpr int STAGES = Q4 && NT == 1 ? 2 : 3;                    // tiles in the ring
   static constexpr bool QREG = NT == 1;               // one query tile: its fragments live in registers
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
     }
   }
   // 4-bit: every p of this warp is held times 2^-ev, so that P s stays within fp16 whatever the steps
-  float ev = -100.f;
+  float ev = -100.f, lim = 0x1p-96f;  // lim: 2^(ev + 4)
 
   uint4 qr[Sh::QREG ? QU : 1];
   uint32_t zq[NT];             // 4-bit: B fragment (k = 2t, 2t + 1) of z sum q: term t of row g's sums, 0 for t = 3
@@ -650,10 +652,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
       built = delta;
     }
 
+    // every key of the tile visible to every row: nothing to mask
+    const bool tile_inner = md.x >= lo && md.x + Sh::TILE <= hi && md.w + Sh::TILE - 1 <= vis.min_pos &&
+                            (p.window == 0 || md.w > vis.max_pos - p.window || md.w + Sh::TILE <= p.sinks);
 #pragma unroll 1
     for (int sub = 0; sub < Sh::SUB; ++sub) {
     const int key0 = (warp * Sh::SUB + sub) * KB, j0 = md.x + key0, kp0 = md.w + key0;  // this step's keys
-    if (j0 >= hi || j0 + KB <= lo) continue;
+    if (!tile_inner && (j0 >= hi || j0 + KB <= lo)) continue;
 
     // ---- scores S^T (times hm: base 2): rows g, g + 8 of each 16-key tile, columns 2t, 2t + 1
     float s[MB][NT][4];
@@ -727,8 +732,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
     }
 
     // ---- masks: only blocks at the ends of an interval or across a row's position or window need them
-    const bool inner = j0 >= lo && j0 + KB <= hi && kp0 + KB - 1 <= vis.min_pos &&
-                       (p.window == 0 || kp0 > vis.max_pos - p.window || kp0 + KB <= p.sinks);
+    const bool inner = tile_inner || (j0 >= lo && j0 + KB <= hi && kp0 + KB - 1 <= vis.min_pos &&
+                                      (p.window == 0 || kp0 > vis.max_pos - p.window || kp0 + KB <= p.sinks));
     if (!inner) {
 #pragma unroll
       for (int u = 0; u < MB; ++u)
@@ -791,15 +796,16 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
         if constexpr (MB == 2) mx = fmaxf(mx, fmaxf(s[1][nt][c], s[1][nt][2 + c]));
         over |= mx > th[nt][c];
       }
-    if constexpr (Sh::Q4) over |= big > __int_as_float(((int)ev + 4 + 127) << 23);
+    if constexpr (Sh::Q4) over |= big > lim;
     if (__any_sync(0xffffffffu, over)) {
       float f = 1.f;
       if constexpr (Sh::Q4) {
         const float wb = warp_max(big);
-        if (wb > __int_as_float(((int)ev + 4 + 127) << 23)) {
-          const float ne = (float)min(max((int)(__float_as_uint(wb) >> 23) - 127, -100), 120);
-          f = ex2(ev - ne);
-          ev = ne;
+        if (wb > lim) {
+          const int ne = min(max((int)(__float_as_uint(wb) >> 23) - 127, -100), 120);
+          f = ex2(ev - (float)ne);
+          ev = (float)ne;
+          lim = __int_as_float((ne + 4 + 127) << 23);
         }
       }
 #pragma unroll
@@ -1263,6 +1269,15 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
   }
   const auto pick = [&](auto d, auto bits) {
     constexpr int DD = decltype(d)::value, BB = decltype(bits)::value;
+    // One tile over a 4-bit cache: with work for every slot of three CTAs an SM their eight more warps pay (64 requests
+    // of 4001-16001 tokens: 234 us, with two CTAs 246); with less, the two CTAs' registers do (8 requests of 2100: 12.1
+    // us, with three 16.0; 16 windowed ones 52 and 78).
+    if constexpr (BB == 4) {
+      if (rows <= 8 && num_seqs * Hkv < 3 * gemm_num_sms()) {
+        launch_rows<DD, BB, 1, 2>(p, kv.size(0) * 2 * Hkv * PS, num_seqs, max_q_len, keys, st);
+        return;
+      }
+    }
     if (rows <= 8)
       launch_rows<DD, BB, 1, 3>(p, kv.size(0) * 2 * Hkv * PS, num_seqs, max_q_len, keys, st);
     else if (rows <= 16 || (DD == 128 && BB == 16))
