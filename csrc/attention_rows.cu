@@ -19,16 +19,24 @@
 //   sum_d q_d (s c_d + z) = s sum_d q_d c_d + z sum_d q_d
 // per group of 64: K runs through the MMA as codes, s touches only the 16 x 8
 // scores and z sum q comes from one more MMA (z is bf16; the sums of the rounded
-// queries are held as three bf16 terms).  For V, s is folded into P; a second
-// MMA with the constant -8 in place of the codes makes them c - 8 (a mean of 7.5
-// would drown long sums), and sum_n p_n (8 s_n + z_n) is kept as one fp32 scalar
-// per group and row, from the unrounded p, so the rounding of P s meets only the
-// deviation s (c - 8).
+// queries are held as three bf16 terms).  For V, s is folded into P and a step's
+// products start from one MMA per group with -8 in place of the codes, so that
+// they sum s (c - 8): the MMA truncates its fp32 sums, and a mean of 7.5 carried
+// through a long context would bias them.  Steps are added in fp32.  The value
+// of code 8, sum_n p_n (8 s_n + z_n), is kept as one fp32 scalar per group and
+// row, from the unrounded p, so the rounding of P s meets only the deviation.
 // Rounding: queries are held in fp16 after scaling each row by a power of two
 // to [2^10, 2^11) (elements 2^-25 below the row's largest are lost), P s in
 // fp16 scaled by a power of two common to the warp; scores, softmax sums and
 // outputs are fp32.  With a bf16 cache the rotated query is split into two bf16
 // terms (hi + lo, 16 bits) and P is rounded to bf16 once.
+//
+// Measured on a B200 (GPU time, head_dim 128): a 4-bit cache is read at 4.0-4.2
+// TB/s with every SM busy and is bound by issue: taking the codes apart (K 40, V
+// 48 logic instructions for 16 keys, on a pipe of half rate) and the softmax; the
+// ring alone, without consumers, brings 6.7 TB/s.  A bf16 cache (32 windowed
+// requests) is read at 6.2 TB/s.  A call's fixed time is about 6.5 us: four
+// dependent reads of the plan, the first tile, one step, the join.
 //
 // The keys that a tile can see (the sink part and the window part of every
 // segment) are split over the CTAs of a thread-block cluster, whose partial
@@ -69,6 +77,12 @@ constexpr float ROWS_M0 = -1e37f;  // running maximum before any visible key (fi
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));                                  \
   }
 BRAID_MMA(mma_f16, "f16")
+// D = A B + C, fp16 operands
+BRAID_DEVICE void mma_f16_c(float* d, const float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 BRAID_MMA(mma_bf16, "bf16")
 #undef BRAID_MMA
 // Transpose of an 8 x 8 matrix of 16-bit elements held across the warp.
@@ -256,7 +270,7 @@ BRAID_DEVICE RowsPiece rows_piece(const RowsParams& p, const RowsWalk& w, int la
     x.n = x.at >= a && x.at < b ? 16 : 0;
   }
   if (x.n > 0) {
-    const int idx = min((w.sl + x.at) / p.PS, w.npages - 1);
+    const int idx = max(min((w.sl + x.at) / p.PS, w.npages - 1), 0);
     x.ofs = (w.sl + x.at) % p.PS;
     x.page = w.pages[idx];
   }
@@ -625,6 +639,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
       for (int c = 0; c < 2; ++c) th[nt][c] = m[nt][c] == ROWS_M0 ? ROWS_M0 : (m[nt][c] + 8.f) / hm[nt][c];
   };
   // The first segment's delta (most plans have one for all) while the first copies are under way.
+  uint32_t m8[4];  // opaque, or the compiler would rebuild them for every use
+  asm volatile("mov.b32 %0, %2; mov.b32 %1, %3;" : "=r"(m8[0]), "=r"(m8[1]) : "n"(NIB_LO_M8), "n"(NIB_HI_M8));
+  m8[2] = m8[0];
+  m8[3] = m8[1];
   bool ok = true;
   int built = nseg > 0 ? segs.delta[0] : 0;
   if (warp < ROWS_WARPS) build(built, xq);
@@ -657,286 +675,308 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
                             (p.window == 0 || md.w > vis.max_pos - p.window || md.w + Sh::TILE <= p.sinks);
 #pragma unroll 1
     for (int sub = 0; sub < Sh::SUB; ++sub) {
-    const int key0 = (warp * Sh::SUB + sub) * KB, j0 = md.x + key0, kp0 = md.w + key0;  // this step's keys
-    if (!tile_inner && (j0 >= hi || j0 + KB <= lo)) continue;
+      const int key0 = (warp * Sh::SUB + sub) * KB, j0 = md.x + key0, kp0 = md.w + key0;  // this step's keys
+      if (!tile_inner && (j0 >= hi || j0 + KB <= lo)) continue;
 
-    // ---- scores S^T (times hm: base 2): rows g, g + 8 of each 16-key tile, columns 2t, 2t + 1
-    float s[MB][NT][4];
-    if constexpr (Sh::Q4) {
-#pragma unroll
-      for (int u = 0; u < MB; ++u) {
-        uint32_t kw[2][QU], kz[2][GR];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = key0 + 16 * u + g + 8 * r;
-          if constexpr (D == 128) {
-            const uint4 v = lds128(kt + key * 64 + t * 16);
-            kw[r][0] = v.x; kw[r][1] = v.y; kw[r][2] = v.z; kw[r][3] = v.w;
-            const uint2 z = lds64(kt + Sh::KS_AT + key * 8);
-            kz[r][0] = z.x; kz[r][1] = z.y;
-          } else {
-            const uint2 v = lds64(kt + key * 32 + t * 8);
-            kw[r][0] = v.x; kw[r][1] = v.y;
-            kz[r][0] = lds32(kt + Sh::KS_AT + key * 4);
-          }
-        }
-        float sa[NT][GR][4];
-#pragma unroll
-        for (int k = 0; k < QU; ++k) {
-          const uint32_t wa = kw[0][k], wb = kw[1][k];
-          const uint32_t a0[4] = {nib_lo(wa), nib_lo(wb), nib_hi(wa), nib_hi(wb)};
-          const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
-          const uint32_t a1[4] = {nib_lo(wa8), nib_lo(wb8), nib_hi(wa8), nib_hi(wb8)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            uint4 q;
-            if constexpr (Sh::QREG) q = qr[k];
-            else q = lds128(qf + ((nt * QU + k) * 32 + lane) * 16);
-            if (k < GR) mma_f16_0(sa[nt][Sh::group(k)], a0, q.x, q.y);
-            else mma_f16(sa[nt][Sh::group(k)], a0, q.x, q.y);
-            mma_f16(sa[nt][Sh::group(k)], a1, q.z, q.w);
-          }
-        }
-        // z of both groups, at k = 2t, 2t + 1 of the rows g and g + 8 (zero at k >= 8 and, through zq, at k 6 and 7)
-        const uint32_t az[4] = {GR == 2 ? __byte_perm(kz[0][0], kz[0][GR - 1], 0x7632) : kz[0][0] >> 16,
-                                GR == 2 ? __byte_perm(kz[1][0], kz[1][GR - 1], 0x7632) : kz[1][0] >> 16, 0u, 0u};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16_0(s[u][nt], az, zq[nt], 0u);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int h = 0; h < GR; ++h) s[u][nt][e] = fmaf(kv4_scale(kz[e >> 1][h]), sa[nt][h][e], s[u][nt][e]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < MB; ++u)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
-#pragma unroll
-      for (int k = 0; k < QU; ++k)
+      // ---- scores S^T (times hm: base 2): rows g, g + 8 of each 16-key tile, columns 2t, 2t + 1
+      float s[MB][NT][4];
+      if constexpr (Sh::Q4) {
 #pragma unroll
         for (int u = 0; u < MB; ++u) {
-          uint32_t a[4];
-          ldsm_x4(kt + Sh::chunk(key0 + 16 * u + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * k + (lane >> 4)), a[0], a[1], a[2], a[3]);
+          uint32_t kw[2][QU], kz[2][GR];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int key = key0 + 16 * u + g + 8 * r;
+            if constexpr (D == 128) {
+              const uint4 v = lds128(kt + key * 64 + t * 16);
+              kw[r][0] = v.x; kw[r][1] = v.y; kw[r][2] = v.z; kw[r][3] = v.w;
+              const uint2 z = lds64(kt + Sh::KS_AT + key * 8);
+              kz[r][0] = z.x; kz[r][1] = z.y;
+            } else {
+              const uint2 v = lds64(kt + key * 32 + t * 8);
+              kw[r][0] = v.x; kw[r][1] = v.y;
+              kz[r][0] = lds32(kt + Sh::KS_AT + key * 4);
+            }
+          }
+          float sa[NT][GR][4];
+#pragma unroll
+          for (int k = 0; k < QU; ++k) {
+            const uint32_t wa = kw[0][k], wb = kw[1][k];
+            const uint32_t a0[4] = {nib_lo(wa), nib_lo(wb), nib_hi(wa), nib_hi(wb)};
+            const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+            const uint32_t a1[4] = {nib_lo(wa8), nib_lo(wb8), nib_hi(wa8), nib_hi(wb8)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint4 q;
+              if constexpr (Sh::QREG) q = qr[k];
+              else q = lds128(qf + ((nt * QU + k) * 32 + lane) * 16);
+              if (k < GR) mma_f16_0(sa[nt][Sh::group(k)], a0, q.x, q.y);
+              else mma_f16(sa[nt][Sh::group(k)], a0, q.x, q.y);
+              mma_f16(sa[nt][Sh::group(k)], a1, q.z, q.w);
+            }
+          }
+          // z of both groups, at k = 2t, 2t + 1 of the rows g and g + 8 (zero at k >= 8 and, through zq, at k 6 and 7)
+          const uint32_t az[4] = {GR == 2 ? __byte_perm(kz[0][0], kz[0][GR - 1], 0x7632) : kz[0][0] >> 16,
+                                  GR == 2 ? __byte_perm(kz[1][0], kz[1][GR - 1], 0x7632) : kz[1][0] >> 16, 0u, 0u};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint4 q;
-            if constexpr (Sh::QREG) q = qr[k];
-            else q = lds128(qf + ((nt * QU + k) * 32 + lane) * 16);
-            mma_bf16(s[u][nt], a, q.z, q.w);
-            mma_bf16(s[u][nt], a, q.x, q.y);
+            mma_bf16_0(s[u][nt], az, zq[nt], 0u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int h = 0; h < GR; ++h) s[u][nt][e] = fmaf(kv4_scale(kz[e >> 1][h]), sa[nt][h][e], s[u][nt][e]);
           }
         }
-    }
-
-    // ---- masks: only blocks at the ends of an interval or across a row's position or window need them
-    const bool inner = tile_inner || (j0 >= lo && j0 + KB <= hi && kp0 + KB - 1 <= vis.min_pos &&
-                                      (p.window == 0 || kp0 > vis.max_pos - p.window || kp0 + KB <= p.sinks));
-    if (!inner) {
+      } else {
 #pragma unroll
-      for (int u = 0; u < MB; ++u)
+        for (int u = 0; u < MB; ++u)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = 16 * u + g + 8 * (e >> 1);
-            const int j = j0 + d, kp = kp0 + d, rp = rpos[nt][e & 1];
-            const bool see = j >= lo && j < hi && kp <= rp && (p.window == 0 || rp - kp < p.window || kp < p.sinks);
-            if (!see) s[u][nt][e] = -INFINITY;
+        for (int k = 0; k < QU; ++k)
+#pragma unroll
+          for (int u = 0; u < MB; ++u) {
+            uint32_t a[4];
+            ldsm_x4(kt + Sh::chunk(key0 + 16 * u + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * k + (lane >> 4)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint4 q;
+              if constexpr (Sh::QREG) q = qr[k];
+              else q = lds128(qf + ((nt * QU + k) * 32 + lane) * 16);
+              mma_bf16(s[u][nt], a, q.z, q.w);
+              mma_bf16(s[u][nt], a, q.x, q.y);
+            }
           }
-    }
+      }
 
-    // ---- 4-bit: (s, z) words of V's keys; keys outside the interval may hold anything
-    [[maybe_unused]] uint32_t vz[MB][2][GR];
-    float big = 0.f;  // largest V step
-    if constexpr (Sh::Q4) {
-#pragma unroll
-      for (int u = 0; u < MB; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = key0 + 16 * u + g + 8 * r;
-          if constexpr (GR == 2) {
-            const uint2 z2 = lds64(kt + Sh::VS_AT + key * 8);
-            vz[u][r][0] = z2.x;
-            vz[u][r][GR - 1] = z2.y;
-          } else {
-            vz[u][r][0] = lds32(kt + Sh::VS_AT + key * 4);
-          }
-        }
+      // ---- masks: only blocks at the ends of an interval or across a row's position or window need them
+      const bool inner = tile_inner || (j0 >= lo && j0 + KB <= hi && kp0 + KB - 1 <= vis.min_pos &&
+                                        (p.window == 0 || kp0 > vis.max_pos - p.window || kp0 + KB <= p.sinks));
       if (!inner) {
 #pragma unroll
         for (int u = 0; u < MB; ++u)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int j = j0 + 16 * u + g + 8 * r;
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < GR; ++h) vz[u][r][h] = j >= lo && j < hi ? vz[u][r][h] : 0u;
-          }
+            for (int e = 0; e < 4; ++e) {
+              const int d = 16 * u + g + 8 * (e >> 1);
+              const int j = j0 + d, kp = kp0 + d, rp = rpos[nt][e & 1];
+              const bool see = j >= lo && j < hi && kp <= rp && (p.window == 0 || rp - kp < p.window || kp < p.sinks);
+              if (!see) s[u][nt][e] = -INFINITY;
+            }
       }
-      __nv_bfloat162 top = __float2bfloat162_rn(0.f);  // packed maximum of the (s, z) words; its s half counts
-#pragma unroll
-      for (int u = 0; u < MB; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int h = 0; h < GR; ++h) top = __hmax2(top, *reinterpret_cast<const __nv_bfloat162*>(&vz[u][r][h]));
-      big = __low2float(top);
-    }
 
-    // ---- running maxima move only when a score passes one by 2^8 (P then stays below 2^8 in its 16-bit type), the
-    // power of two of P s only when a step passes 2^4 times what it was set for
-    bool over = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float mx = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
-        if constexpr (MB == 2) mx = fmaxf(mx, fmaxf(s[1][nt][c], s[1][nt][2 + c]));
-        over |= mx > th[nt][c];
-      }
-    if constexpr (Sh::Q4) over |= big > lim;
-    if (__any_sync(0xffffffffu, over)) {
-      float f = 1.f;
+      // ---- 4-bit: (s, z) words of V's keys; keys outside the interval may hold anything
+      [[maybe_unused]] uint32_t vz[MB][2][GR];
+      float big = 0.f;  // largest V step
       if constexpr (Sh::Q4) {
-        const float wb = warp_max(big);
-        if (wb > lim) {
-          const int ne = min(max((int)(__float_as_uint(wb) >> 23) - 127, -100), 120);
-          f = ex2(ev - (float)ne);
-          ev = (float)ne;
-          lim = __int_as_float((ne + 4 + 127) << 23);
+#pragma unroll
+        for (int u = 0; u < MB; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int key = key0 + 16 * u + g + 8 * r;
+            if constexpr (GR == 2) {
+              const uint2 z2 = lds64(kt + Sh::VS_AT + key * 8);
+              vz[u][r][0] = z2.x;
+              vz[u][r][GR - 1] = z2.y;
+            } else {
+              vz[u][r][0] = lds32(kt + Sh::VS_AT + key * 4);
+            }
+          }
+        if (!inner) {
+#pragma unroll
+          for (int u = 0; u < MB; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int j = j0 + 16 * u + g + 8 * r;
+#pragma unroll
+              for (int h = 0; h < GR; ++h) vz[u][r][h] = j >= lo && j < hi ? vz[u][r][h] : 0u;
+            }
         }
+        __nv_bfloat162 top = __float2bfloat162_rn(0.f);  // packed maximum of the (s, z) words; its s half counts
+#pragma unroll
+        for (int u = 0; u < MB; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int h = 0; h < GR; ++h) top = __hmax2(top, *reinterpret_cast<const __nv_bfloat162*>(&vz[u][r][h]));
+        big = __low2float(top);
       }
+
+      // ---- running maxima move only when a score passes one by 2^8 (P then stays below 2^8 in its 16-bit type), the
+      // power of two of P s only when a step passes 2^4 times what it was set for
+      bool over = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float mx = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
           if constexpr (MB == 2) mx = fmaxf(mx, fmaxf(s[1][nt][c], s[1][nt][2 + c]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = mx == -INFINITY ? m[nt][c] : fmaxf(m[nt][c], mx * hm[nt][c]);
-          const float corr = ex2(m[nt][c] - mx) * f;
-          m[nt][c] = mx;
-          mb[nt][c] = (mx == ROWS_M0 ? 0.f : mx) + (Sh::Q4 ? ev : 0.f);
-          th[nt][c] = mx == ROWS_M0 ? ROWS_M0 : (mx + 8.f) / hm[nt][c];
-          l[nt][c] *= corr;
-#pragma unroll
-          for (int h = 0; h < GR; ++h) rest[nt][h][c] *= corr;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            acc[nt][i][c] *= corr;
-            acc[nt][i][2 + c] *= corr;
+          over |= mx > th[nt][c];
+        }
+      if constexpr (Sh::Q4) over |= big > lim;
+      if (__any_sync(0xffffffffu, over)) {
+        float f = 1.f;
+        if constexpr (Sh::Q4) {
+          const float wb = warp_max(big);
+          if (wb > lim) {
+            const int ne = min(max((int)(__float_as_uint(wb) >> 23) - 127, -100), 120);
+            f = ex2(ev - (float)ne);
+            ev = (float)ne;
+            lim = __int_as_float((ne + 4 + 127) << 23);
           }
         }
-    }
-
-    // ---- P and O^T += V^T P^T
-    const auto weigh = [&](auto masked) {
-      constexpr bool MASK = decltype(masked)::value;
 #pragma unroll
-      for (int u = 0; u < MB; ++u) {
-        uint32_t pb[NT][GR][2];
-        [[maybe_unused]] float sv[2][GR], zv[2][GR];  // V's steps and the values of code 8
-        if constexpr (Sh::Q4) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+            if constexpr (MB == 2) mx = fmaxf(mx, fmaxf(s[1][nt][c], s[1][nt][2 + c]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = mx == -INFINITY ? m[nt][c] : fmaxf(m[nt][c], mx * hm[nt][c]);
+            const float corr = ex2(m[nt][c] - mx) * f;
+            m[nt][c] = mx;
+            mb[nt][c] = (mx == ROWS_M0 ? 0.f : mx) + (Sh::Q4 ? ev : 0.f);
+            th[nt][c] = mx == ROWS_M0 ? ROWS_M0 : (mx + 8.f) / hm[nt][c];
+            l[nt][c] *= corr;
 #pragma unroll
-            for (int h = 0; h < GR; ++h) {
-              sv[r][h] = kv4_scale(vz[u][r][h]);
-              zv[r][h] = fmaf(8.f, sv[r][h], kv4_offset(vz[u][r][h]));
+            for (int h = 0; h < GR; ++h) rest[nt][h][c] *= corr;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              acc[nt][i][c] *= corr;
+              acc[nt][i][2 + c] *= corr;
             }
           }
-        }
+      }
+
+      // ---- P and O^T += V^T P^T
+      const auto weigh = [&](auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        uint32_t pq[MB][NT][GR][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float pr[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pr[e] = ex2(fmaf(s[u][nt][e], hm[nt][e & 1], -mb[nt][e & 1]));
-            l[nt][e & 1] += pr[e];
-          }
+        for (int u = 0; u < MB; ++u) {
+          auto& pb = pq[u];
+          [[maybe_unused]] float sv[2][GR], zv[2][GR];  // V's steps and the values of code 8
           if constexpr (Sh::Q4) {
 #pragma unroll
-            for (int h = 0; h < GR; ++h) {
-              float ps[4];
+            for (int r = 0; r < 2; ++r) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float sc = sv[e >> 1][h], zc = zv[e >> 1][h];
-                // a masked score has weight 0, and 0 times NaN would not be 0
-                const bool skip = MASK && s[u][nt][e] == -INFINITY;
-                ps[e] = skip ? 0.f : pr[e] * sc;
-                rest[nt][h][e & 1] = fmaf(pr[e], skip ? 0.f : zc, rest[nt][h][e & 1]);
+              for (int h = 0; h < GR; ++h) {
+                sv[r][h] = kv4_scale(vz[u][r][h]);
+                zv[r][h] = fmaf(8.f, sv[r][h], kv4_offset(vz[u][r][h]));
               }
-              pb[nt][h][0] = movmatrix_t(pack_f16(ps[0], ps[1]));
-              pb[nt][h][1] = movmatrix_t(pack_f16(ps[2], ps[3]));
             }
-          } else {
-            pb[nt][0][0] = movmatrix_t(pack_bf16(pr[0], pr[1]));
-            pb[nt][0][1] = movmatrix_t(pack_bf16(pr[2], pr[3]));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float pr[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              pr[e] = ex2(fmaf(s[u][nt][e], hm[nt][e & 1], -mb[nt][e & 1]));
+              l[nt][e & 1] += pr[e];
+            }
+            if constexpr (Sh::Q4) {
+#pragma unroll
+              for (int h = 0; h < GR; ++h) {
+                float ps[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float sc = sv[e >> 1][h], zc = zv[e >> 1][h];
+                  // a masked score has weight 0, and 0 times NaN would not be 0
+                  const bool skip = MASK && s[u][nt][e] == -INFINITY;
+                  ps[e] = skip ? 0.f : pr[e] * sc;
+                  rest[nt][h][e & 1] = fmaf(pr[e], skip ? 0.f : zc, rest[nt][h][e & 1]);
+                }
+                pb[nt][h][0] = movmatrix_t(pack_f16(ps[0], ps[1]));
+                pb[nt][h][1] = movmatrix_t(pack_f16(ps[2], ps[3]));
+              }
+            } else {
+              pb[nt][0][0] = movmatrix_t(pack_bf16(pr[0], pr[1]));
+              pb[nt][0][1] = movmatrix_t(pack_bf16(pr[2], pr[3]));
+            }
+          }
+          if constexpr (!Sh::Q4) {
+            uint32_t keep[2] = {~0u, ~0u};  // keys 2t, 2t + 1 and 2t + 8, 2t + 9: those outside the interval read as 0
+            if constexpr (MASK) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int j = j0 + 16 * u + 2 * t + (r & 1) + 8 * (r >> 1);
+                if (j < lo || j >= hi) keep[r >> 1] &= (r & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              uint32_t a[4];
+              ldsm_x4_t(kt + Sh::V_AT + Sh::chunk(key0 + 16 * u + (lane & 7) + (lane >> 4) * 8, 2 * i + ((lane >> 3) & 1)), a[0],
+                        a[1], a[2], a[3]);
+              if constexpr (MASK) {
+                a[0] &= keep[0];
+                a[1] &= keep[0];
+                a[2] &= keep[1];
+                a[3] &= keep[1];
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt][i], a, pb[nt][0][0], pb[nt][0][1]);
+            }
           }
         }
         if constexpr (Sh::Q4) {
           constexpr int NV = D / 64;
-          uint32_t vw[4][NV];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the tile
+          float low[NT][GR][4];  // -8 P of the step: what every MMA tile of a group starts from
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = key0 + 16 * u + 2 * t + (r & 1) + 8 * (r >> 1);
-            if constexpr (D == 128) {
-              const uint2 v = lds64(kt + Sh::V_AT + key * 64 + g * 8);
-              vw[r][0] = v.x; vw[r][1] = v.y;
-            } else {
-              vw[r][0] = lds32(kt + Sh::V_AT + key * 32 + g * 4);
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < GR; ++h) {
+              mma_f16_0(low[nt][h], m8, pq[0][nt][h][0], pq[0][nt][h][1]);
+              if constexpr (MB == 2) mma_f16(low[nt][h], m8, pq[MB - 1][nt][h][0], pq[MB - 1][nt][h][1]);
             }
-          }
+          uint32_t vw[MB][4][NV];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of each 16
 #pragma unroll
-          for (int k = 0; k < NV; ++k) {
-            const uint32_t x0 = __byte_perm(vw[0][k], vw[1][k], 0x5410), y0 = __byte_perm(vw[0][k], vw[1][k], 0x7632);
-            const uint32_t x1 = __byte_perm(vw[2][k], vw[3][k], 0x5410), y1 = __byte_perm(vw[2][k], vw[3][k], 0x7632);
-            const uint32_t a8[4] = {x0, x0 >> 8, y0, y0 >> 8}, b8[4] = {x1, x1 >> 8, y1, y1 >> 8};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t a[4] = {nib_lo(a8[i]), nib_hi(a8[i]), nib_lo(b8[i]), nib_hi(b8[i])};
-              const uint32_t m8[4] = {NIB_LO_M8, NIB_HI_M8, NIB_LO_M8, NIB_HI_M8};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_f16(acc[nt][k * 4 + i], a, pb[nt][Sh::group(k)][0], pb[nt][Sh::group(k)][1]);
-                mma_f16(acc[nt][k * 4 + i], m8, pb[nt][Sh::group(k)][0], pb[nt][Sh::group(k)][1]);
-              }
-            }
-          }
-        } else {
-          uint32_t keep[2] = {~0u, ~0u};  // keys 2t, 2t + 1 and 2t + 8, 2t + 9: those outside the interval read as 0
-          if constexpr (MASK) {
+          for (int u = 0; u < MB; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int j = j0 + 16 * u + 2 * t + (r & 1) + 8 * (r >> 1);
-              if (j < lo || j >= hi) keep[r >> 1] &= (r & 1) ? 0x0000FFFFu : 0xFFFF0000u;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            uint32_t a[4];
-            ldsm_x4_t(kt + Sh::V_AT + Sh::chunk(key0 + 16 * u + (lane & 7) + (lane >> 4) * 8, 2 * i + ((lane >> 3) & 1)), a[0],
-                      a[1], a[2], a[3]);
-            if constexpr (MASK) {
-              a[0] &= keep[0];
-              a[1] &= keep[0];
-              a[2] &= keep[1];
-              a[3] &= keep[1];
+              const int key = key0 + 16 * u + 2 * t + (r & 1) + 8 * (r >> 1);
+              if constexpr (D == 128) {
+                const uint2 v = lds64(kt + Sh::V_AT + key * 64 + g * 8);
+                vw[u][r][0] = v.x; vw[u][r][1] = v.y;
+              } else {
+                vw[u][r][0] = lds32(kt + Sh::V_AT + key * 32 + g * 4);
+              }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt][i], a, pb[nt][0][0], pb[nt][0][1]);
-          }
+          for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {  // halves of the words: MMA tiles 2 hf, 2 hf + 1
+              uint32_t x[MB][2];
+#pragma unroll
+              for (int u = 0; u < MB; ++u) {
+                x[u][0] = __byte_perm(vw[u][0][k], vw[u][1][k], hf ? 0x7632 : 0x5410);
+                x[u][1] = __byte_perm(vw[u][2][k], vw[u][3][k], hf ? 0x7632 : 0x5410);
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float d[4];
+#pragma unroll
+                  for (int u = 0; u < MB; ++u) {
+                    const uint32_t y0 = i ? x[u][0] >> 8 : x[u][0], y1 = i ? x[u][1] >> 8 : x[u][1];
+                    const uint32_t av[4] = {nib_lo(y0), nib_hi(y0), nib_lo(y1), nib_hi(y1)};
+                    if (u == 0) mma_f16_c(d, low[nt][Sh::group(k)], av, pq[u][nt][Sh::group(k)][0], pq[u][nt][Sh::group(k)][1]);
+                    else mma_f16(d, av, pq[u][nt][Sh::group(k)][0], pq[u][nt][Sh::group(k)][1]);
+                  }
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[nt][k * 4 + hf * 2 + i][e] += d[e];
+                }
+            }
         }
-      }
-    };
-    if (inner)
-      weigh(std::false_type{});
-    else
-      weigh(std::true_type{});
+      };
+      if (inner)
+        weigh(std::false_type{});
+      else
+        weigh(std::true_type{});
 
     }
     // ---- every lane is done with the stage
@@ -957,44 +997,44 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
   const float up = Sh::Q4 ? ex2(ev) : 1.f;
   if (warp < ROWS_WARPS) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float sum = l[nt][c];
+      for (int c = 0; c < 2; ++c) {
+        float sum = l[nt][c];
 #pragma unroll
-      for (int o = 4; o <= 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if constexpr (Sh::Q4) {
+        for (int o = 4; o <= 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if constexpr (Sh::Q4) {
 #pragma unroll
-        for (int h = 0; h < GR; ++h)
+          for (int h = 0; h < GR; ++h)
 #pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) rest[nt][h][c] += __shfl_xor_sync(0xffffffffu, rest[nt][h][c], o);
-      }
-      const int r = nt * 8 + 2 * t + c;
-      if (g == 0) {
-        s_m[warp][r] = m[nt][c];
-        s_l[warp][r] = sum * up;
-      }
-      float* dst = aw + (warp * Sh::ROWS + r) * Sh::LD;
-      if constexpr (Sh::Q4) {
+            for (int o = 4; o <= 16; o <<= 1) rest[nt][h][c] += __shfl_xor_sync(0xffffffffu, rest[nt][h][c], o);
+        }
+        const int r = nt * 8 + 2 * t + c;
+        if (g == 0) {
+          s_m[warp][r] = m[nt][c];
+          s_l[warp][r] = sum * up;
+        }
+        float* dst = aw + (warp * Sh::ROWS + r) * Sh::LD;
+        if constexpr (Sh::Q4) {
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k) {
-          float o8[8];
+          for (int k = 0; k < D / 64; ++k) {
+            float o8[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o8[2 * i] = fmaf(acc[nt][k * 4 + i][c], 0x1p24f, rest[nt][Sh::group(k)][c]) * up;
-            o8[2 * i + 1] = fmaf(acc[nt][k * 4 + i][2 + c], 0x1p20f, rest[nt][Sh::group(k)][c]) * up;
+            for (int i = 0; i < 4; ++i) {
+              o8[2 * i] = fmaf(acc[nt][k * 4 + i][c], 0x1p24f, rest[nt][Sh::group(k)][c]) * up;
+              o8[2 * i + 1] = fmaf(acc[nt][k * 4 + i][2 + c], 0x1p20f, rest[nt][Sh::group(k)][c]) * up;
+            }
+            *reinterpret_cast<float4*>(dst + Sh::v_dim(k, g)) = make_float4(o8[0], o8[1], o8[2], o8[3]);
+            *reinterpret_cast<float4*>(dst + Sh::v_dim(k, g) + 4) = make_float4(o8[4], o8[5], o8[6], o8[7]);
           }
-          *reinterpret_cast<float4*>(dst + Sh::v_dim(k, g)) = make_float4(o8[0], o8[1], o8[2], o8[3]);
-          *reinterpret_cast<float4*>(dst + Sh::v_dim(k, g) + 4) = make_float4(o8[4], o8[5], o8[6], o8[7]);
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          dst[16 * i + g] = acc[nt][i][c];
-          dst[16 * i + g + 8] = acc[nt][i][2 + c];
+          for (int i = 0; i < MT; ++i) {
+            dst[16 * i + g] = acc[nt][i][c];
+            dst[16 * i + g + 8] = acc[nt][i][2 + c];
+          }
         }
       }
-    }
   }
   __syncthreads();
   constexpr int C4 = D / 4;
@@ -1204,6 +1244,7 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
     TORCH_CHECK(kv.is_cuda() && kv.scalar_type() == at::kBFloat16 && kv.dim() == 5 && kv.is_contiguous() &&
                     kv.size(1) == 2 && reinterpret_cast<uintptr_t>(kv.data_ptr()) % 16 == 0,
                 "attention: cache must be a contiguous bf16 tensor [P, 2, Hkv, page, D]");
+    TORCH_CHECK(kv.numel() / D < (1ll << 31), "attention: a bf16 cache of more than 2^31 rows");
   }
   const at::cuda::CUDAGuard guard(dev);
   const bool given = out_arg.has_value() && out_arg->defined();

@@ -170,6 +170,28 @@ def test_without_rope_and_gpt2_heads(bits):
 
 
 @pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_segments(bits, d):
+    """More segments than the kernel keeps in shared memory, each with its own RoPE delta."""
+    seqs = [(1, [(5 + j % 3, j % 16, j % 7) for j in range(90)]), (3, [(7, 0, -(j % 3)) for j in range(70)] + [(3, 0, 0)]),
+            (1, [(0, 0, 0)] * 80 + [(4, 0, 0)])]
+    _against_definition(bits, d, 4, 2, 16, seqs, 300, 9, pages=400)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_negative_scale_and_zero_queries(bits):
+    d = 128
+    meta, T = make_plan([(1, [(200, 0, 0)]), (1, [(33, 0, 0)])], 16, 64, DEV)
+    cache, kv = _pool(bits, 64, 2, 16, d)
+    q = torch.randn(T, 8, d, device=DEV, generator=_gen(3)).bfloat16()
+    q[1, 3:6] = 0
+    cos, sin = _tables(d)
+    got = _run(q, cache, meta, d, 100, 2, scale=-0.07)
+    ref = dense64(q, kv, meta, cos, sin, -0.07, 100, 2, base=code8(cache) if bits == 4 else None)
+    check(got, ref, ROWS4 if bits == 4 else ROWS16)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
 @pytest.mark.parametrize("nq", [1, 6])
 def test_rows_that_see_nothing_are_zero(bits, nq):
     d = 128
