@@ -128,13 +128,26 @@ __global__ void __launch_bounds__(256) qkv_prepare_kv4_kernel(const Kv4AppendPar
     unpack8(raw[u], v);
     const __nv_bfloat16* nw = is_q ? p.qn : (is_k ? p.kn : nullptr);
     if (__any_sync(0xffffffffu, nw != nullptr)) {
-      // squares rounded, then summed by neighbours: fours in order, and a tree over them
-      float sq[8];
+      // Squares rounded, then summed by halves: of the fours of neighbours (D 128) or of the elements (D 64), the upper
+      // half onto the lower until one is left, the order of a plain strided reduction; the last steps are in the lane.
+      float sq[8], ss;
 #pragma unroll
       for (int j = 0; j < 8; ++j) sq[j] = __fmul_rn(v[j], v[j]);
-      float ss = (((sq[0] + sq[1]) + sq[2]) + sq[3]) + (((sq[4] + sq[5]) + sq[6]) + sq[7]);
+      if constexpr (D == 128) {
+        float a = ((sq[0] + sq[1]) + sq[2]) + sq[3], b = ((sq[4] + sq[5]) + sq[6]) + sq[7];
 #pragma unroll
-      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        for (int o = LPH / 2; o > 0; o >>= 1) {
+          a += __shfl_xor_sync(0xffffffffu, a, o);
+          b += __shfl_xor_sync(0xffffffffu, b, o);
+        }
+        ss = a + b;
+      } else {
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sq[j] += __shfl_xor_sync(0xffffffffu, sq[j], o);
+        ss = ((sq[0] + sq[4]) + (sq[2] + sq[6])) + ((sq[1] + sq[5]) + (sq[3] + sq[7]));
+      }
       if (nw != nullptr) {
         const float rstd = rsqrtf(ss / D + p.eps);
         float wt[8];
