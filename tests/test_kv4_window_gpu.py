@@ -370,6 +370,20 @@ def test_tokens_behind_the_last_sequence_are_left_alone():
     assert (out[T:] == 7).all() and (out[:T] != 7).any()
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("nq", [1, 5])
+def test_page_ids_outside_the_pool_stay_inside_it(bits, nq):
+    """The kernel reads the first or the last page instead; the other sequence's rows are what they were."""
+    d = 128
+    meta, T = make_plan([(nq, [(100, 0, 0)]), (nq, [(60, 0, 0)])], 16, 64, DEV)
+    cache, _ = _pool(bits, 64, 2, 16, d)
+    q = torch.randn(T, 8, d, device=DEV, generator=_gen(1)).bfloat16()
+    good = _run(q, cache, meta, d, 200, 1)
+    meta.page_ids[1], meta.page_ids[2] = -7, 64
+    bad = _run(q, cache, meta, d, 200, 1)
+    assert torch.equal(bad[nq:], good[nq:]) and bad.isfinite().all()
+
+
 def test_refusals():
     d = 128
     meta, T = make_plan([(1, [(40, 0, 0)])], 16, 8, DEV)
@@ -418,3 +432,36 @@ def test_engine_graphs_match_eager(extra, tmp_path):
         got.append([o["token_ids"] for o in llm.generate(prompts, sp)])
         llm.exit()
     assert got[0] == got[1]
+
+
+def test_checked_build_records_bad_slots_and_pages():
+    """The bounds-checked build records a slot and a page id outside the 4-bit cache, whose accesses are skipped or held
+    inside in every build."""
+    try:
+        from braidinfer_b200 import _C_checked as C
+    except ImportError:
+        pytest.skip("bounds-checked build not present")
+    from braidinfer_b200.ops import _ext
+    _ext.ext()
+    saved, d = _ext._C, 128
+    _ext._C = _ext._Counted(C)
+    try:
+        C.bounds_check_status()
+        layer = rand_layer4(8, 2, 16, d, 0, DEV)
+        cos, sin = _tables(d)
+        pos = torch.zeros(2, device=DEV, dtype=torch.int32)
+        qkv = torch.randn(2, 12 * d, device=DEV).bfloat16()
+        ops.qkv_prepare(qkv, pos, torch.tensor([3, 128], device=DEV, dtype=torch.int32), layer, 8, 2, d, cos, sin)
+        v = int(C.bounds_check_status())
+        assert (v >> 48, v & 0xFFFFFFFFFFFF) == (1, 128)
+        meta, T = make_plan([(1, [(40, 0, 0)])], 16, 8, DEV)
+        q = torch.randn(T, 8, d, device=DEV).bfloat16()
+        _run(q, layer, meta, d)
+        assert int(C.bounds_check_status()) == 0
+        meta.page_ids[1] = 9
+        _run(q, layer, meta, d)
+        v = int(C.bounds_check_status())
+        assert (v >> 48, v & 0xFFFFFFFFFFFF) == (4, 9)
+    finally:
+        torch.cuda.synchronize()
+        _ext._C = saved
