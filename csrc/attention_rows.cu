@@ -1145,7 +1145,7 @@ static void launch_rows(RowsParams& p, int64_t pool_rows, int64_t num_seqs, int6
                      Sh::SMEM, st, dim3(1, 1, (unsigned)S), tm, p);
 }
 
-// Long prompts (head_dim 128): the tcgen05 prefill kernel of attention_tc.cu with the window.  A 4-bit cache is first
+// Prompts of 512 (token, head) rows and more (head_dim 128): the tcgen05 prefill kernel of attention_tc.cu with the window.  A 4-bit cache is first
 // read into a bf16 workspace, page by page as the plan lists them: one more rounding of K and V to bf16, and 2 + 0.56
 // bytes an element once per call, against the whole prompt's products (4000 tokens of Llama-3-8B heads: 8 of 190 us).
 bool attn_prefill_tc_use(int D, int64_t rows);
@@ -1304,7 +1304,9 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
   int64_t keys = std::max<int64_t>(1, max_kv_len);
   if (window > 0) keys = std::min(keys, window + sinks + max_q_len);
   const int64_t rows = max_q_len * p.G;
-  if (max_q_len > 1 && attn_prefill_tc_use((int)D, T * p.G)) {
+  // From 512 (token, head) rows, half of where the calls without a window and a 4-bit cache change kernels: 128 queries
+  // of 32 heads over 3200 keys 73 us by rows and 61 here (bf16: 119 and 46), 64 queries 46 and 59 (bf16 60 and 49).
+  if (max_q_len > 1 && attn_prefill_tc_use((int)D, 2 * T * p.G)) {
     attention_prompt(p, q4 ? nullptr : &kv, kv, scales, T, num_seqs, max_q_len, keys, page_ids.numel(), st);
     return out;
   }

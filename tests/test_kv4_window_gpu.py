@@ -39,7 +39,7 @@ def _against_definition(bits, d, G, hkv, ps, seqs, window, sinks, rope=True, pag
     got = _run(q, cache, meta, d, window, sinks, rope)
     torch.cuda.synchronize()
     cos, sin = _tables(d)
-    if d == 128 and meta.max_q_len > 1 and T * G >= 1024:  # the long-prompt kernel
+    if d == 128 and meta.max_q_len > 1 and T * G >= 512:  # the long-prompt kernel
         check(got, dense64(q, kv, meta, cos, sin, d ** -0.5, window, sinks, rope), TC4 if bits == 4 else TC16)
     else:
         base = code8(cache) if bits == 4 else None
