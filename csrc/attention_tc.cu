@@ -285,12 +285,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
   // [126] barriers and TMEM set up, [127] first K tile issued
   unsigned long long* trc = p.tc_trace ? p.tc_trace + (size_t)lin * 128 : nullptr;
   if (trc != nullptr && threadIdx.x == 0) trc[62] = globaltimer_ns();
+  // Every CTA waits for the preceding kernels at the latest before its output, also one without rows or keys: else a
+  // grid of such CTAs alone would complete before them, and its successors would not wait for them either.  WIN waits
+  // here, because the kernels right before it may have written the plan, its workspace or its zeroed counters; without
+  // WIN the plan was uploaded before the step's first kernel, and the prologue overlaps the QKV GEMM.
+  if (WIN) pdl_wait();
   const int G = p.G;
   const int t0 = p.qo_indptr[b], nt = p.qo_indptr[b + 1] - t0;
   const int rows = nt * G;
   const int cta_rows = p.cta_rows == TC_ROWS ? TC_ROWS : TC_CTA_ROWS;
   const int row0 = qtile * cta_rows;
-  if (row0 >= rows) return;
+  if (row0 >= rows) {
+    pdl_wait();
+    return;
+  }
   const int nrows = min(cta_rows, rows - row0);
   const int nq = nrows > TC_ROWS ? 2 : 1;  // Q tiles with live rows (CTA-uniform)
   // largest position among the CTA's rows (rows of a shared-prefix group are not ordered)
@@ -610,6 +618,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefill_tc_kernel(const __
       if (have && !mbar_wait(&bar.odone[t], 0)) s_abort = 1;
       tc_fence_after();
       // ------------------------------------------------------------ output
+      if (j == 0) pdl_wait();  // without keys nothing above waited: the output, partials and counters may still be in use
       const bool direct = S == 1 && !p.partial_only;
       const int stride = p.split_stride > 0 ? p.split_stride : S;
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;

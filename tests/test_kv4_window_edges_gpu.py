@@ -1,0 +1,89 @@
+"""4-bit and windowed attention on a GPU where launches, splits, values and batches end."""
+import pytest
+import torch
+from kv4_helpers import ROWS4, ROWS16, TC4, TC16, check, code8, dense64, make_plan, rand_layer4, unpack64
+
+from braidinfer_b200 import ops
+from braidinfer_b200.ops._ext import ext
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+PLAN = ("qo_indptr", "positions", "seg_indptr", "seg_page_indptr", "seg_offset", "seg_len", "seg_pos0", "seg_delta",
+        "page_ids")
+
+
+@pytest.fixture
+def tcgen05():
+    """Calls of several queries with head_dim 128 take the tcgen05 kernel, whatever their size."""
+    ext().attn_select_prefill_tc(1)
+    yield
+    ext().attn_select_prefill_tc(-1)
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _tables(d, n=8192):
+    return ops.build_cos_sin(d, 1e4, n, device=DEV)
+
+
+def _pool(bits, pages, hkv, ps, d, seed=0):
+    """(cache argument, its values fp64)"""
+    if bits == 4:
+        layer = rand_layer4(pages, hkv, ps, d, seed, DEV)
+        return layer, unpack64(layer)
+    kv = torch.randn(pages, 2, hkv, ps, d, device=DEV, generator=_gen(seed)).bfloat16()
+    return kv, kv.double()
+
+
+def _queries(T, hq, d, seed=1):
+    return torch.randn(T, hq, d, device=DEV, generator=_gen(seed)).bfloat16()
+
+
+# ---------------------------------------------------- launches and key splits
+@pytest.mark.parametrize("bits", [4, 16])
+def test_key_splits_without_keys_and_a_plan_written_just_before(bits, tcgen05):
+    """Most key splits of the short sequences have no keys; the plan, the counters that join the splits and the memory of
+    the output are written by the kernels right before the call, and two plans take turns."""
+    d, G, ps, pages = 128, 4, 16, 600
+    seqs = [(150, [(4000, 0, 0)]), (1, [(1, 0, 0)]), (3, [(140, 2, 0)]), (0, [(9, 0, 0)]), (20, [(20, 0, 0)])]
+    plans = [make_plan(seqs, ps, pages, DEV, seed=i, qpos_shift=-7 * i)[0] for i in range(2)]
+    cache, kv = _pool(bits, pages, 1, ps, d)
+    T = 174
+    q = _queries(T, G, d)
+    cos, sin = _tables(d)
+    window = 0 if bits == 4 else 1 << 29
+    call = lambda meta: ops.attention(q, cache, meta, cos, sin, d ** -0.5, window=window)  # noqa: E731
+    alone = []
+    for meta in plans:
+        torch.cuda.synchronize()
+        alone.append(call(meta).clone())
+        check(alone[-1], dense64(q, kv, meta, cos, sin, d ** -0.5, window), TC4 if bits == 4 else TC16)
+    live = make_plan(seqs, ps, pages, DEV, seed=0)[0]
+    outs = []
+    for i in range(40):
+        held = torch.full((T, G * d), float("nan"), device=DEV, dtype=torch.bfloat16)
+        del held  # the call's output takes its place
+        for f in PLAN:
+            getattr(live, f).copy_(getattr(plans[i % 2], f))
+        outs.append(call(live).clone())
+    assert all(torch.equal(o, alone[i % 2]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_a_call_without_any_visible_key_waits_for_what_came_before(bits, tcgen05):
+    """No CTA has a key to load, so none waits for one: the zeros still come after what was written there before."""
+    d, ps = 128, 16
+    meta, T = make_plan([(256, [(0, 0, 0)])], ps, 16, DEV)
+    cache, _ = _pool(bits, 16, 1, ps, d)
+    q = _queries(T, 4, d)
+    cos, sin = _tables(d)
+    for _ in range(20):
+        held = torch.empty(T, 4 * d, device=DEV, dtype=torch.bfloat16)
+        held.fill_(7)
+        del held
+        out = ops.attention(q, cache, meta, cos, sin, d ** -0.5, window=300)
+        after = out + 0
+        assert (out == 0).all() and (after == 0).all()
