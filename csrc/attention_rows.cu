@@ -577,9 +577,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
         ph ^= 1;
       }
     }
-    // no copy may outlive the CTA, also where a consumer gave up
-    if (!ok)
-      for (int j = i - Sh::STAGES; j < i; ++j) (void)mbar_wait(&full_bar[j % Sh::STAGES], (j / Sh::STAGES) & 1);
+    // Tiles [0, i) were issued.  No copy may outlive the CTA or land in the space of the partial results, also where this
+    // warp or a consumer gave up, so those not known to have landed are waited for.  Tile i - STAGES is known where the
+    // loop ended regularly: the consumers released its stage to the end mark, whose arrival is that barrier's next phase.
+    for (int j = max(0, i - Sh::STAGES + (ok ? 1 : 0)); j < i; ++j)
+      (void)mbar_wait(&full_bar[j % Sh::STAGES], (j / Sh::STAGES) & 1);
   }
   // ---------------------------------------------------------------- consumers
   float acc[NT][MT][4];

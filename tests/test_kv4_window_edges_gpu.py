@@ -87,3 +87,29 @@ def test_a_call_without_any_visible_key_waits_for_what_came_before(bits, tcgen05
         out = ops.attention(q, cache, meta, cos, sin, d ** -0.5, window=300)
         after = out + 0
         assert (out == 0).all() and (after == 0).all()
+
+
+# --------------------------------------------------------- tiles of the ring
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq", [1, 4])
+def test_every_number_of_tiles(bits, d, nq):
+    """0 to 9 tiles of 64 or 128 keys in a CTA: fewer than the ring holds, as many, and more, so that the producer ends at
+    every stage and phase.  Many sequences in one call, so that keys are not split."""
+    hkv, G, ps = 2, 4, 16
+    lens = [n for k in range(10) for n in (64 * k, 64 * k + 1)]
+    seqs = [(nq, [(max(n, 1), 0, 0)]) for n in lens] * 12
+    pages = sum(-(-max(n, 1) // ps) for n in lens) * 12
+    meta, T = make_plan(seqs, ps, pages, DEV, qpos_shift=0)
+    cache, kv = _pool(bits, pages, hkv, ps, d)
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    window = 0 if bits == 4 else 1 << 29
+    # of d 128 and several queries a sequence, the row kernel whatever the size of the batch
+    ext().attn_select_prefill_tc(0)
+    try:
+        got = ops.attention(q, cache, meta, cos, sin, d ** -0.5, window=window)
+    finally:
+        ext().attn_select_prefill_tc(-1)
+    ref = dense64(q, kv, meta, cos, sin, d ** -0.5, window, base=code8(cache) if bits == 4 else None)
+    check(got, ref, ROWS4 if bits == 4 else ROWS16)
