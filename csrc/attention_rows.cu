@@ -1253,7 +1253,7 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
   const torch::Tensor out = given ? *out_arg : at::empty({T, Hq * D}, q.options());
   TORCH_CHECK(kv.device() == dev && out.device() == dev, "attention: q, cache and out on different devices");
   const int64_t Hkv = kv.size(2), PS = kv.size(3);
-  TORCH_CHECK(kv.size(4) == (q4 ? D / 2 : D) && Hkv > 0 && Hq % Hkv == 0, "attention: head layout mismatch");
+  TORCH_CHECK(kv.size(4) == (q4 ? D / 2 : D) && Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention: head layout mismatch");
   TORCH_CHECK(PS > 0 && PS % 16 == 0 && kv.size(0) > 0, "attention: page size must be a multiple of 16, the pool not empty");
   TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.numel() == T * Hq * D,
               "attention: out must be a contiguous bf16 [T, Hq * D]");

@@ -331,6 +331,7 @@ void kv4_check_layer(const torch::Tensor& codes, const torch::Tensor& scales, co
   TORCH_CHECK(scales.device() == codes.device(), who, ": codes and scales on different devices");
   const int64_t D = codes.size(4) * 2;
   TORCH_CHECK(D == 64 || D == 128, who, ": 4-bit cache head_dim must be 64 or 128");
+  TORCH_CHECK(codes.size(2) > 0, who, ": 4-bit cache without KV heads");
   TORCH_CHECK(codes.size(1) == 2 && scales.size(0) == codes.size(0) && scales.size(1) == 2 &&
                   scales.size(2) == codes.size(2) && scales.size(3) == codes.size(3) &&
                   scales.size(4) == D / KV4_GROUP && scales.size(5) == 2,
@@ -361,7 +362,7 @@ torch::Tensor qkv_prepare_kv4(const torch::Tensor& qkv, const torch::Tensor& pos
                   qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(1) == 1 && qkv.stride(0) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
               who, ": qkv must be a bf16 [T, (Hq + 2 Hkv) D] tensor with 16-byte aligned rows on the device of the cache");
-  TORCH_CHECK(codes.size(2) == Hkv && codes.size(4) * 2 == D, who, ": cache layout mismatch");
+  TORCH_CHECK(Hq >= 0 && codes.size(2) == Hkv && codes.size(4) * 2 == D, who, ": cache layout mismatch");
   const int64_t T = qkv.size(0);
   const bool has_qn = q_norm.has_value() && q_norm->defined(), has_kn = k_norm.has_value() && k_norm->defined();
   const at::cuda::CUDAGuard g(dev);

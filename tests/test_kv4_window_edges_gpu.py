@@ -113,3 +113,29 @@ def test_every_number_of_tiles(bits, d, nq):
         ext().attn_select_prefill_tc(-1)
     ref = dense64(q, kv, meta, cos, sin, d ** -0.5, window, base=code8(cache) if bits == 4 else None)
     check(got, ref, ROWS4 if bits == 4 else ROWS16)
+
+
+# ------------------------------------------------------------------ refusals
+def test_head_counts_that_leave_nothing_are_refused():
+    d, P, ps = 128, 4, 16
+    empty = ops.KV4Layer(torch.zeros(P, 2, 0, ps, d // 2, dtype=torch.uint8, device=DEV),
+                         torch.zeros(P, 2, 0, ps, d // 64, 2, dtype=torch.bfloat16, device=DEV))
+    full = rand_layer4(P, 2, ps, d, 0, DEV)
+    i = torch.zeros(3, dtype=torch.int32, device=DEV)
+    cos, sin = _tables(d)
+    qkv = torch.zeros(3, 2 * d, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        ops.kv4_read(empty, i)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        ops.qkv_prepare(qkv, i, i, empty, 2, 0, d, cos, sin)
+    with pytest.raises(RuntimeError, match="layout"):  # -2 + 2 * 2 heads are as wide as qkv
+        ops.qkv_prepare(qkv, i, i, full, -2, 2, d, cos, sin)
+    meta, T = make_plan([(1, [(20, 0, 0)])], ps, P, DEV)
+    with pytest.raises(RuntimeError, match="head layout"):
+        ops.attention(torch.zeros(T, 0, d, dtype=torch.bfloat16, device=DEV), full, meta, cos, sin, 0.1)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        ops.attention(_queries(T, 4, d), empty, meta, cos, sin, 0.1)
+    # no query heads to append with, and no tokens, are calls like any other
+    assert ops.qkv_prepare(torch.zeros(1, 4 * d, dtype=torch.bfloat16, device=DEV), i[:1], i[:1], full, 0, 2, d, cos,
+                           sin).shape == (1, 0, d)
+    assert ops.kv4_read(full, i[:0]).shape == (0, 2, 2, d)
