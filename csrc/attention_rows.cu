@@ -1255,8 +1255,9 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
   const int64_t Hkv = kv.size(2), PS = kv.size(3);
   TORCH_CHECK(kv.size(4) == (q4 ? D / 2 : D) && Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention: head layout mismatch");
   TORCH_CHECK(PS > 0 && PS % 16 == 0 && kv.size(0) > 0, "attention: page size must be a multiple of 16, the pool not empty");
-  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.numel() == T * Hq * D,
-              "attention: out must be a contiguous bf16 [T, Hq * D]");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.numel() == T * Hq * D &&
+                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+              "attention: out must be a contiguous, 16-byte aligned bf16 [T, Hq * D]");
   TORCH_CHECK(window >= 0 && window < (1ll << 30) && sinks >= 0 && sinks < (1ll << 30),
               "attention: window and sinks must be in [0, 2^30)");
   TORCH_CHECK(num_seqs >= 0 && max_q_len >= 0 && max_q_len <= T, "attention: max_q_len must be in [0, T]");
@@ -1285,8 +1286,10 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
   if (use_rope) {
     TORCH_CHECK(cos.device() == dev && sin.device() == dev && cos.scalar_type() == at::kFloat &&
                     sin.scalar_type() == at::kFloat && cos.is_contiguous() && sin.is_contiguous() && cos.dim() == 2 &&
-                    cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes(),
-                "attention: cos and sin must be contiguous fp32 [positions, D/2] tables on the device of the cache");
+                    cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes() &&
+                    reinterpret_cast<uintptr_t>(cos.data_ptr()) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(sin.data_ptr()) % 16 == 0,
+                "attention: cos and sin must be contiguous, 16-byte aligned fp32 [positions, D/2] tables on the device of the cache");
     p.cos = cos.data_ptr<float>();
     p.sin = sin.data_ptr<float>();
     p.rope_len = (int)cos.size(0);

@@ -379,8 +379,10 @@ torch::Tensor qkv_prepare_kv4(const torch::Tensor& qkv, const torch::Tensor& pos
   if (use_rope)
     TORCH_CHECK(cos.device() == dev && sin.device() == dev && cos.scalar_type() == at::kFloat &&
                     sin.scalar_type() == at::kFloat && cos.is_contiguous() && sin.is_contiguous() && cos.dim() == 2 &&
-                    cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes(),
-                who, ": cos and sin must be contiguous fp32 [positions, D/2] tables on the device of the cache");
+                    cos.size(1) == D / 2 && cos.size(0) >= 1 && sin.sizes() == cos.sizes() &&
+                    reinterpret_cast<uintptr_t>(cos.data_ptr()) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(sin.data_ptr()) % 16 == 0,
+                who, ": cos and sin must be contiguous, 16-byte aligned fp32 [positions, D/2] tables on the device of the cache");
   Kv4AppendParams p{};
   p.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
   p.q_out = has_qn ? reinterpret_cast<__nv_bfloat16*>(q_out.data_ptr()) : nullptr;

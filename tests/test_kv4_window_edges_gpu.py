@@ -139,3 +139,31 @@ def test_head_counts_that_leave_nothing_are_refused():
     assert ops.qkv_prepare(torch.zeros(1, 4 * d, dtype=torch.bfloat16, device=DEV), i[:1], i[:1], full, 0, 2, d, cos,
                            sin).shape == (1, 0, d)
     assert ops.kv4_read(full, i[:0]).shape == (0, 2, 2, d)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("nq", [1, 300])
+def test_tables_and_outputs_that_are_not_aligned_are_refused(bits, nq):
+    """Contiguous tables one element into their storage: the kernels read them 16 bytes at a time."""
+    d, ps, P = 128, 16, 64
+    meta, T = make_plan([(nq, [(400, 0, 0)])], ps, P, DEV)
+    cache, _ = _pool(bits, P, 2, ps, d)
+    q = _queries(T, 8, d)
+    cos, sin = _tables(d, 512)
+    off = torch.empty(cos.numel() + 1, device=DEV)[1:].view_as(cos)
+    off.copy_(cos)
+    assert off.is_contiguous()
+    for c, s in ((off, sin), (cos, off)):
+        with pytest.raises(RuntimeError, match="aligned"):
+            ops.attention(q, cache, meta, c, s, 0.1, window=100)
+        if bits == 4:
+            i = torch.zeros(1, dtype=torch.int32, device=DEV)
+            with pytest.raises(RuntimeError, match="aligned"):
+                ops.qkv_prepare(torch.zeros(1, 12 * d, dtype=torch.bfloat16, device=DEV), i, i, cache, 8, 2, d, c, s)
+    out = torch.empty(T * 8 * d + 1, dtype=torch.bfloat16, device=DEV)[1:].view(T, 8 * d)
+    kv, scales = cache if bits == 4 else (cache, None)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ext().attention_rows(out, q, kv, scales, *(getattr(meta, f) for f in PLAN), cos, sin, 0.1, True, 1, nq, 400, 100, 0)
+    # a table that starts at a later row is aligned
+    got = ops.attention(q, cache, meta, cos[1:], sin[1:], 0.1, window=100)
+    assert torch.equal(got, ops.attention(q, cache, meta, cos[1:].clone(), sin[1:].clone(), 0.1, window=100))
