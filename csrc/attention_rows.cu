@@ -1182,7 +1182,8 @@ static void attention_prompt(const RowsParams& r, const torch::Tensor* pool, con
   p.sin = r.sin;
   p.rope_len = r.rope_len;
   p.use_rope = r.use_rope;
-  p.scale_log2 = r.scale_log2 * r.q_sign;
+  p.scale_log2 = r.scale_log2;
+  p.q_flip = r.q_sign < 0.f ? 0x80008000u : 0u;
   p.Hq = r.Hq;
   p.Hkv = r.Hkv;
   p.G = r.G;

@@ -177,6 +177,13 @@ BRAID_DEVICE void tc_build_q_row(const AttnParams& p, uint8_t* qs, int r, bool l
     qa[c] = live ? __ldg(reinterpret_cast<const uint4*>(qp + c * 8)) : make_uint4(0, 0, 0, 0);
     qb[c] = live ? __ldg(reinterpret_cast<const uint4*>(qp + 64 + c * 8)) : make_uint4(0, 0, 0, 0);
   }
+  if (p.q_flip != 0) {  // masks and maxima want a positive scale
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      qa[c].x ^= p.q_flip; qa[c].y ^= p.q_flip; qa[c].z ^= p.q_flip; qa[c].w ^= p.q_flip;
+      qb[c].x ^= p.q_flip; qb[c].y ^= p.q_flip; qb[c].z ^= p.q_flip; qb[c].w ^= p.q_flip;
+    }
+  }
   if (live && p.use_rope) {
     int pos = rpos - delta;
     pos = pos < 0 ? 0 : (pos >= p.rope_len ? p.rope_len - 1 : pos);

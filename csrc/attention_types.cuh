@@ -53,6 +53,7 @@ struct AttnParams {
   int window;                 // tcgen05 prefill: positions a query sees back from its own (0: no window) ...
   int sinks;                  // ... and the first positions it always sees
   int page_identity;          // tcgen05 prefill: page i of the plan's list is page i of the pool
+  uint32_t q_flip;            // tcgen05 prefill: 0x80008000 to negate the queries (a negative scale), else 0
   const int* seq_nsh;         // decode: 1 for sequences of the shared-prefix group (nullptr: none)
 };
 

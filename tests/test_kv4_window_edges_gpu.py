@@ -167,3 +167,20 @@ def test_tables_and_outputs_that_are_not_aligned_are_refused(bits, nq):
     # a table that starts at a later row is aligned
     got = ops.attention(q, cache, meta, cos[1:], sin[1:], 0.1, window=100)
     assert torch.equal(got, ops.attention(q, cache, meta, cos[1:].clone(), sin[1:].clone(), 0.1, window=100))
+
+
+# ------------------------------------------------------------ scales and NaN
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("scale", [-0.07, -1.5, 1e-30, 0.0])
+def test_any_scale_in_the_tcgen05_kernel(bits, rope, scale, tcgen05):
+    """Masked scores, maxima and edge tiles under a negative scale; a scale of 0 weighs every visible key alike."""
+    d, G, hkv, ps, pages = 128, 4, 2, 16, 200
+    seqs = [(300, [(700, 3, 0), (300, 0, 0)]), (40, [(40, 0, 0)]), (1, [(900, 0, 2)])]
+    meta, T = make_plan(seqs, ps, pages, DEV)
+    cache, kv = _pool(bits, pages, hkv, ps, d)
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    got = ops.attention(q, cache, meta, cos, sin, scale, rope, window=500, sinks=3)
+    ref = dense64(q, kv, meta, cos, sin, scale, 500, 3, rope)
+    check(got, ref, TC4 if bits == 4 else TC16)
