@@ -21,7 +21,11 @@ without its per-page Python loop.
 With ``window`` W > 0 it must also hold that ``p - (seg_pos0[s] + j) < W`` or
 ``seg_pos0[s] + j < sinks``: the last W positions (the query's own among them)
 and the first ``sinks`` positions of the composition.  A query that sees no key
-gets zeros.  Slots that no query of a tile sees may hold anything, NaN included.
+gets zeros.  Slots that no query of a sequence sees may hold anything, NaN
+included.  On CUDA, with a window or a 4-bit cache, a NaN in a query or in a key
+that it sees makes its row NaN; one in a V row of a bf16 cache, or with many
+queries of either, may also reach those queries of the sequence that do not see
+it (weight 0 times NaN).
 
 The cache may also be a 4-bit one (``kv4.KV4Layer``): same pages, slots and plan.
 

@@ -1013,7 +1013,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
         }
         const int r = nt * 8 + 2 * t + c;
         if (g == 0) {
-          s_m[warp][r] = m[nt][c];
+          // a sum that is NaN counts even if no score of the warp was a number, which leaves the maximum where it was
+          s_m[warp][r] = sum != sum && m[nt][c] == ROWS_M0 ? 0.f : m[nt][c];
           s_l[warp][r] = sum * up;
         }
         float* dst = aw + (warp * Sh::ROWS + r) * Sh::LD;

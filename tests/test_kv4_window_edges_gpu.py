@@ -184,3 +184,44 @@ def test_any_scale_in_the_tcgen05_kernel(bits, rope, scale, tcgen05):
     got = ops.attention(q, cache, meta, cos, sin, scale, rope, window=500, sinks=3)
     ref = dense64(q, kv, meta, cos, sin, scale, 500, 3, rope)
     check(got, ref, TC4 if bits == 4 else TC16)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq", [1, 6, 300])
+def test_a_visible_nan_reaches_its_rows_and_no_other(bits, d, nq):
+    """A NaN query, or a NaN in a key that a row sees, makes the row NaN, also where no other key of it is a number or
+    where the other keys are other warps' and CTAs'; the other rows are what they were."""
+    ps, hkv, G = 16, 2, 4
+    lens = [1, 17, 33, 129, 3001]
+    seqs = [(min(nq, n), [(n, 0, 0)]) for n in lens]
+    pages = sum(-(-n // ps) for n in lens)
+    meta, T = make_plan(seqs, ps, pages, DEV)
+    cache, kv = _pool(bits, pages, hkv, ps, d)
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    window = 0 if bits == 4 else 1 << 29
+    run = lambda q, c: ops.attention(q, c, meta, cos, sin, d ** -0.5, window=window).view(T, hkv * G, d)  # noqa: E731
+    clean = run(q, cache)
+    assert clean.isfinite().all()
+    h = meta.host
+    first = [int(i) for i in h["qo_indptr"]]
+    qn = q.clone()  # head 3 of each sequence's last token
+    last = [i - 1 for i in first[1:]]
+    qn[last, 3, 5] = float("nan")
+    out = run(qn, cache)
+    assert out[last, 3].isnan().all()
+    out[last, 3] = clean[last, 3]
+    assert torch.equal(out, clean)
+    for b, n in enumerate(lens):  # the last key of one sequence after the other: only the last token sees it
+        page, slot = int(h["page_ids"][int(h["seg_page_indptr"][b]) + (n - 1) // ps]), (n - 1) % ps
+        if bits == 4:
+            bad = ops.KV4Layer(cache.codes, cache.scales.clone())
+            bad.scales[page, 0, 1, slot] = float("nan")
+        else:
+            bad = cache.clone()
+            bad[page, 0, 1, slot, 7] = float("nan")
+        out = run(q, bad)
+        assert out[last[b], G:].isnan().all(), n
+        out[last[b], G:] = clean[last[b], G:]
+        assert torch.equal(out, clean), n
