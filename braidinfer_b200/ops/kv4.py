@@ -19,6 +19,10 @@ elements takes 72 bytes instead of 256.
 A row of codes is ``D / 8`` little-endian 32-bit words; word ``2 i + h`` holds
 elements ``8 i + h D / 2`` and the seven after it, element ``j`` in bits
 ``4 j .. 4 j + 3`` (the order in which the attention kernels read them).
+
+Attention over the cache on CUDA takes rotated query elements up to 2**100 in
+magnitude, steps of V from 2**-60 on (0 included) and, where a group of V is
+constant, values up to 2**50; beyond that its sums may overflow or lose bits.
 """
 from __future__ import annotations
 

@@ -27,9 +27,12 @@
 // row, from the unrounded p, so the rounding of P s meets only the deviation.
 // Rounding: queries are held in fp16 after scaling each row by a power of two
 // to [2^10, 2^11) (elements 2^-25 below the row's largest are lost), P s in
-// fp16 scaled by a power of two common to the warp; scores, softmax sums and
-// outputs are fp32.  With a bf16 cache the rotated query is split into two bf16
-// terms (hi + lo, 16 bits) and P is rounded to bf16 once.
+// fp16 scaled by a power of two common to the warp, that of the largest step it
+// has met (elements 2^-25 below that are lost); scores, softmax sums and outputs
+// are fp32.  This holds for rotated query elements up to 2^100, steps of V from
+// 2^-60 and constant groups of V (step 0) up to 2^50; above that, sums may
+// overflow, below that, bits are lost.  With a bf16 cache the rotated query is
+// split into two bf16 terms (hi + lo, 16 bits) and P is rounded to bf16 once.
 //
 // Measured on a B200 (GPU time, head_dim 128): a 4-bit cache is read at 4.0-4.2
 // TB/s with every SM busy and is bound by issue: taking the codes apart (K 40, V
@@ -59,6 +62,7 @@ namespace braid {
 constexpr int ROWS_WARPS = 4;                       // consumer warps
 constexpr int ROWS_THREADS = 32 * (ROWS_WARPS + 1);  // and the producer
 constexpr int ROWS_END = INT_MIN;                   // description of the tile after the last
+constexpr float ROWS_EV0 = -50.f;  // first exponent that the weights over a 4-bit cache are held times
 constexpr float ROWS_M0 = -1e37f;  // running maximum before any visible key (finite: differences stay defined)
 
 // D (+)= A (16 x 16) B (16 x 8), fp32 accumulation, fp16 or bf16 operands.  Plain (not volatile) asm: the compiler
@@ -598,8 +602,9 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
       for (int h = 0; h < GR; ++h) rest[nt][h][c] = 0.f;
     }
   }
-  // 4-bit: every p of this warp is held times 2^-ev, so that P s stays within fp16 whatever the steps
-  float ev = -100.f, lim = 0x1p-96f;  // lim: 2^(ev + 4)
+  // 4-bit: every p of this warp is held times 2^-ev, so that P s stays within fp16 whatever the steps; from -50 on, so
+  // that sums of p (8 s + z) stay within fp32 where no step moves it (constant groups have step 0)
+  float ev = ROWS_EV0, lim = 0x1p-46f;  // lim: 2^(ev + 4)
 
   uint4 qr[Sh::QREG ? QU : 1];
   uint32_t zq[NT];             // 4-bit: B fragment (k = 2t, 2t + 1) of z sum q: term t of row g's sums, 0 for t = 3
@@ -822,7 +827,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
         if constexpr (Sh::Q4) {
           const float wb = warp_max(big);
           if (wb > lim) {
-            const int ne = min(max((int)(__float_as_uint(wb) >> 23) - 127, -100), 120);
+            const int ne = min((int)(__float_as_uint(wb) >> 23) - 127, 120);  // above ROWS_EV0 + 3
             f = ex2(ev - (float)ne);
             ev = (float)ne;
             lim = __int_as_float((ne + 4 + 127) << 23);

@@ -225,3 +225,42 @@ def test_a_visible_nan_reaches_its_rows_and_no_other(bits, d, nq):
         assert out[last[b], G:].isnan().all(), n
         out[last[b], G:] = clean[last[b], G:]
         assert torch.equal(out, clean), n
+
+
+# --------------------------------------------- the ends of the 4-bit V range
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq", [1, 4])
+@pytest.mark.parametrize("value", [0.0, -1000.0, 2.0 ** 30, -2.0 ** 45])
+def test_constant_v_groups(d, nq, value):
+    """Groups of one value have step 0: nothing moves the scale of P, and the offsets alone are summed, over scores that
+    rise by nearly 2^8 without moving the maximum."""
+    ps, hkv, G, n = 16, 1, 8 // nq if nq < 8 else 1, 3000
+    pages = -(-n // ps) + 1
+    meta, T = make_plan([(nq, [(n, 0, 0)])], ps, pages, DEV)
+    layer = ops.KV4Cache(1, pages, hkv, ps, d, device=DEV)[0]
+    h = meta.host
+    kp = torch.zeros(pages, ps, device=DEV)
+    for j in range(n):
+        kp[int(h["page_ids"][j // ps]), j % ps] = j
+    # K constant along D: score k d / d = k, in base 2 from 0 to 7.8 after the first 256 keys
+    layer.scales[:, 0, :, :, :, 1] = torch.where(kp >= 256, 5.4, 0.0)[:, None, :, None].bfloat16()
+    layer.scales[:, 1, :, :, :, 1] = value
+    q = torch.ones(T, hkv * G, d, device=DEV, dtype=torch.bfloat16)
+    cos, sin = _tables(d)
+    got = ops.attention(q, layer, meta, cos, sin, 1.0 / d, use_rope=False)
+    assert ((got.double() - value).abs() <= (2 ** -8 + 2 ** -15) * abs(value)).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq", [1, 4])
+@pytest.mark.parametrize("exponent", [-45, 60, 110])
+def test_v_steps_far_from_one(d, nq, exponent):
+    ps, hkv, G, pages = 16, 2, 4, 64
+    seqs = [(nq, [(300, 0, 0)]), (nq, [(40, 3, 0)])]
+    meta, T = make_plan(seqs, ps, pages, DEV)
+    layer = rand_layer4(pages, hkv, ps, d, 0, DEV)
+    layer.scales[:, 1] *= 2.0 ** exponent
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    got = ops.attention(q, layer, meta, cos, sin, d ** -0.5)
+    check(got, dense64(q, unpack64(layer), meta, cos, sin, d ** -0.5, base=code8(layer)), ROWS4)
