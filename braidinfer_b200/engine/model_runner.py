@@ -114,6 +114,20 @@ class ModelRunner:
             row = self.spec.head_dim * torch.tensor([], dtype=self.dtype).element_size()
         return 2 * self.spec.num_layers * L.kv_heads * self.page_size * row
 
+    def attention_workspace_bytes(self) -> int:
+        """What the attention of many queries over a 4-bit cache may allocate: its plan's pages as bf16, up to the ops'
+        limit, once for eager steps and once for the prefill graphs (of one sequence and the padding one)."""
+        if self.config.kv_cache_dtype != "int4" or self.device.type != "cuda" or self.spec.head_dim != 128:
+            return 0
+        from ..ops._ext import ext
+
+        limit = int(ext().attn_kv4_workspace_limit())
+        page = 2 * self.model.layout.kv_heads * self.page_size * self.spec.head_dim * 2
+        cfg = self.config
+        pages = self._graph_caps(1)[1] + 1
+        graphs = cfg.use_cuda_graphs and self._prefill_bucket(1) > 0
+        return min(limit, cfg.max_num_seqs * pages * page) + (min(limit, pages * page) if graphs else 0)
+
     def auto_num_pages(self) -> int:
         cfg = self.config
         if cfg.num_kvcache_blocks > 0:
@@ -122,7 +136,7 @@ class ModelRunner:
             return 64
         free, total = torch.cuda.mem_get_info(self.device)
         used = total - free
-        act = cfg.max_num_batched_tokens * self.spec.hidden_size * 64 + (2 << 30)
+        act = cfg.max_num_batched_tokens * self.spec.hidden_size * 64 + (2 << 30) + self.attention_workspace_bytes()
         budget = total * cfg.gpu_memory_utilization - used - act
         n = int(budget // self.kv_bytes_per_page())
         if self.tp.size > 1:

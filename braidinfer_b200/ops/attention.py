@@ -241,9 +241,13 @@ def attention(q: torch.Tensor, kv_layer: Union[torch.Tensor, KV4Layer], meta: At
     window, and ``sinks`` without one changes nothing).
 
     A :class:`KV4Layer` or a window takes its own kernels
-    (``csrc/attention_rows.cu``): decode or not follows from the rows, keys are
-    split inside the kernel without a workspace, ``meta.num_splits`` is not
-    used, and a plan with a shared-prefix group is refused."""
+    (``csrc/attention_rows.cu``): decode or not follows from the rows,
+    ``meta.num_splits`` is not used, and a plan with a shared-prefix group is
+    refused.  Calls of few rows a sequence split keys inside the kernel without a
+    workspace.  With many rows a sequence and head_dim 128 the call may allocate
+    partial results and, of a 4-bit cache, the plan's pages as bf16 (at most
+    ``ext().attn_kv4_workspace_limit()`` bytes; a plan that would need more takes
+    the kernel without); queries and such pages are then rounded to bf16."""
     window, sinks = int(window), int(sinks)
     if window < 0 or sinks < 0 or window >= 1 << 30 or sinks >= 1 << 30:
         raise ValueError(f"attention: window and sinks must be in [0, 2**30), got {window} and {sinks}")

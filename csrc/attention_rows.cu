@@ -1114,6 +1114,31 @@ int gemm_num_sms();
 unsigned long long* next_span(const char* name);
 void kv4_check_layer(const torch::Tensor& codes, const torch::Tensor& scales, const char* who);
 
+// Key parts per row tile, and about how long the call then takes.
+struct RowsPlan {
+  int splits;
+  int64_t ns;
+};
+
+// A power of two up to the 16 CTAs of a cluster, each part of at least one tile: the fewest waves of resident CTAs times
+// (its keys' time + the fixed time of a CTA: plan, queries, first tile, joining).  Fitted on a B200 (head_dim 128): with
+// every slot busy a CTA takes 17 ns a key from a 4-bit cache, from a bf16 one 24 ns with three CTAs an SM (one row tile)
+// and 14 with one, and 8 us apart from its keys.  64 requests of 10000 keys: 288, 254, 259, 302 us at 1, 2, 4, 8 parts;
+// 8 requests of 2100: 28, 22, 17, 24 us; one request of 600 on 8 KV heads: 10.7, 9.5, 8.2, 7.2 us.  `work`: row tiles of
+// all sequences and KV heads.
+template <int D, int BITS, int NT, int OCC>
+static RowsPlan rows_plan(int64_t work, int64_t max_keys) {
+  using Sh = RowsShape<D, BITS, NT>;
+  const int64_t slots = (int64_t)std::min(OCC, (int)(227 * 1024 / (Sh::SMEM + 4096))) * gemm_num_sms();
+  const int64_t per_key = (Sh::Q4 ? 17 : NT == 1 ? 24 : 14) * D / 128;  // ns
+  RowsPlan best{1, INT64_MAX};
+  for (int n = 1; n <= 16 && (n == 1 || max_keys >= (int64_t)n * Sh::TILE / 2); n *= 2) {
+    const int64_t est = (work * n + slots - 1) / slots * (max_keys / n * per_key + 8000);
+    if (est < best.ns) best = {n, est};
+  }
+  return best;
+}
+
 template <int D, int BITS, int NT, int OCC>
 static void launch_rows(RowsParams& p, int64_t pool_rows, int64_t num_seqs, int64_t max_q, int64_t max_keys, cudaStream_t st) {
   using Sh = RowsShape<D, BITS, NT>;
@@ -1127,23 +1152,7 @@ static void launch_rows(RowsParams& p, int64_t pool_rows, int64_t num_seqs, int6
     ready[dev & 63] = true;
   }
   const int64_t tiles = (max_q * p.G + Sh::ROWS - 1) / Sh::ROWS;
-  const int64_t work = tiles * num_seqs * p.Hkv;
-  // Key parts per tile, a power of two up to the 16 CTAs of a cluster, each of at least one tile: the fewest waves of
-  // resident CTAs times (its keys' time + the fixed time of a CTA: plan, queries, first tile, joining).  Fitted on a
-  // B200: with every slot busy a CTA takes 17 ns a key from a 4-bit cache and 24 ns from a bf16 one (head_dim 128), and
-  // 8 us apart from its keys.  64 requests of 10000 keys: 288, 254, 259, 302 us at 1, 2, 4, 8 parts; 8 requests of 2100:
-  // 28, 22, 17, 24 us; one request of 600 on 8 KV heads: 10.7, 9.5, 8.2, 7.2 us.
-  const int64_t slots = (int64_t)std::min(OCC, (int)(227 * 1024 / (Sh::SMEM + 4096))) * gemm_num_sms();
-  const int64_t per_key = (Sh::Q4 ? 17 : 24) * D / 128;  // ns
-  int S = 1;
-  int64_t best = INT64_MAX;
-  for (int n = 1; n <= 16 && (n == 1 || max_keys >= (int64_t)n * Sh::TILE / 2); n *= 2) {
-    const int64_t est = (work * n + slots - 1) / slots * (max_keys / n * per_key + 8000);
-    if (est < best) {
-      best = est;
-      S = n;
-    }
-  }
+  const int S = rows_plan<D, BITS, NT, OCC>(tiles * num_seqs * p.Hkv, max_keys).splits;
   p.splits = S;
   p.whole = Sh::Q4 && p.PS % Sh::TILE == 0;
   TORCH_CHECK(tiles < (1ll << 31) && num_seqs <= 65535 && (int64_t)p.Hkv * S <= 65535, "attention: launch grid too large");
@@ -1153,15 +1162,72 @@ static void launch_rows(RowsParams& p, int64_t pool_rows, int64_t num_seqs, int6
                      Sh::SMEM, st, dim3(1, 1, (unsigned)S), tm, p);
 }
 
-// Prompts of 512 (token, head) rows and more (head_dim 128): the tcgen05 prefill kernel of attention_tc.cu with the window.  A 4-bit cache is first
-// read into a bf16 workspace, page by page as the plan lists them: one more rounding of K and V to bf16, and 2 + 0.56
-// bytes an element once per call, against the whole prompt's products (4000 tokens of Llama-3-8B heads: 8 of 190 us).
-bool attn_prefill_tc_use(int D, int64_t rows);
+// Calls of many rows a sequence (head_dim 128): the tcgen05 prefill kernel of attention_tc.cu with the window.  A 4-bit
+// cache is first read into a bf16 workspace, page by page as the plan lists them: one more rounding of K and V to bf16,
+// and 2 + 0.56 bytes an element once per call, against the whole prompt's products (4000 tokens of Llama-3-8B heads: 8 of
+// 190 us).
+int attn_prefill_tc_mode();
 int attn_prefill_tc_rows();
 int attn_prefill_tc_min_rows();
 void launch_attn_prefill_tc(const AttnParams& p, int num_seqs, int max_q_len, int64_t P, cudaStream_t st);
 void kv4_unpack_pages(torch::Tensor out, const torch::Tensor& codes, const torch::Tensor& scales, const RowsParams& p,
                       int64_t num_seqs, cudaStream_t st);
+
+// Query rows per CTA as for the calls without a window: 128 where CTAs of 256 would fill less than half of the SMs.
+static int prompt_cta_rows(int64_t max_rows, int64_t num_seqs, int64_t Hkv) {
+  const int64_t units = (max_rows + attn_prefill_tc_rows() - 1) / attn_prefill_tc_rows() * num_seqs * Hkv;
+  return units * 2 <= gemm_num_sms() ? attn_prefill_tc_min_rows() : attn_prefill_tc_rows();
+}
+
+// Key splits of that kernel, where its row tiles (`units`, of all sequences and KV heads) leave SMs idle, and about how
+// long the call then takes in units of a 128-key tile: waves of (tiles and about two of prologue), and the join.
+struct PromptPlan {
+  int splits;
+  int64_t tiles;
+};
+static PromptPlan prompt_plan(int64_t units, int64_t keys) {
+  const int64_t sms = gemm_num_sms(), kvt = std::max<int64_t>(1, (keys + 127) / 128);
+  PromptPlan best{1, (units + sms - 1) / sms * (kvt + 2)};
+  for (int n = 2; n <= 32 && n <= kvt && units < sms; ++n) {
+    const int64_t est = (units * n + sms - 1) / sms * ((kvt + n - 1) / n + 2) + n;
+    if (est < best.tiles) best = {n, est};
+  }
+  return best;
+}
+
+// The largest workspace that a call over a 4-bit cache takes; one that would need more goes by rows.
+constexpr int64_t PROMPT_WORKSPACE = 2ll << 30;
+int64_t attn_kv4_workspace_limit() { return PROMPT_WORKSPACE; }
+
+// Whether a call of several queries takes the tcgen05 kernel.  By rows of the sequences, not of the batch: a sequence's
+// rows are taken 16 at a time by the row kernel and up to 256 at a time by that one, whose tile costs the same however
+// few they are, and from a 4-bit cache every listed page is written and read once more first.  The shorter of the two
+// estimates decides: rows_plan() and a tile of 2.3 us, 8 us of prologue and output, and from a 4-bit cache 6 us and
+// 0.14 ns a key and KV head (what a B200 measured with 4 heads on each of 8 KV heads).  By rows and by tcgen05, us:
+//   queries x sequences over keys    4-bit cache        bf16 cache
+//    64 x 1 over  3200                41    56           55    46
+//   128 x 1 over  3200                67    60          108    44
+//     2 x 64 over 3200                87   447          135   224
+//    16 x 16 over 3200               131   120          223    61
+//    64 x 16 over 3200               453   133          748    73
+//    32 x 1 over 12000                68    85           99    63
+// Sequences of unequal length count by their rows together, a tile more for each.
+// A prompt of 512 rows takes the tcgen05 kernel also where that is up to 20 us slower (512 rows over 600 keys in 4 bits:
+// 21 and 30), so that prompts round alike whatever their length.
+static bool prompt_pays(bool q4, int64_t T, int64_t num_seqs, int64_t max_q_len, int64_t G, int64_t Hkv, int64_t PS,
+                        int64_t keys, int64_t num_page_ids) {
+  const int64_t max_rows = max_q_len * G, slots = num_page_ids * PS * Hkv;
+  if (q4 && slots * 2 * 128 * 2 > PROMPT_WORKSPACE) return false;
+  if (attn_prefill_tc_mode() >= 0) return attn_prefill_tc_mode() == 1;
+  if (max_rows <= 8) return false;  // one row tile
+  const auto tiles = [&](int64_t rows) {
+    return std::min((max_rows + rows - 1) / rows * num_seqs, T * G / rows + num_seqs) * Hkv;
+  };
+  const int64_t by_rows = q4 ? rows_plan<128, 4, 2, 2>(tiles(16), keys).ns : rows_plan<128, 16, 2, 2>(tiles(16), keys).ns;
+  const int64_t units = tiles(prompt_cta_rows(max_rows, num_seqs, Hkv));
+  const int64_t here = 8000 + prompt_plan(units, keys).tiles * 2300 + (q4 ? 6000 + slots * 14 / 100 : 0);
+  return here < by_rows + (max_rows >= 512 ? 20000 : 0);
+}
 
 static void attention_prompt(const RowsParams& r, const torch::Tensor* pool, const torch::Tensor& kv,
                              const c10::optional<torch::Tensor>& scales, int64_t T, int64_t num_seqs, int64_t max_q_len,
@@ -1198,26 +1264,11 @@ static void attention_prompt(const RowsParams& r, const torch::Tensor* pool, con
   p.window = r.window > 0 ? r.window : 1 << 30;
   p.sinks = r.window > 0 ? r.sinks : 0;
   p.span = r.span;
-  // as for the calls without a window: 128-row CTAs where 256-row ones would fill less than half of the SMs, key
-  // splits where the row tiles leave SMs idle.  The join's counters belong to this call alone.
-  const int64_t sms = gemm_num_sms();
-  const int64_t w256 = (max_q_len * r.G + attn_prefill_tc_rows() - 1) / attn_prefill_tc_rows() * num_seqs * r.Hkv;
-  p.cta_rows = w256 * 2 <= sms ? attn_prefill_tc_min_rows() : attn_prefill_tc_rows();
-  const int64_t qt = (max_q_len * r.G + p.cta_rows - 1) / p.cta_rows, work_units = qt * num_seqs * r.Hkv;
-  p.num_splits = 1;
-  if (work_units < sms) {
-    const int64_t kvt = std::max<int64_t>(1, (keys + 127) / 128);
-    int64_t best = INT64_MAX;
-    for (int n = 1; n <= 32 && n <= kvt; ++n) {
-      const int64_t est = ((work_units * n + sms - 1) / sms) * ((kvt + n - 1) / n + 2) + (n > 1 ? n : 0);
-      if (est < best) {
-        best = est;
-        p.num_splits = n;
-      }
-    }
-  }
+  p.cta_rows = prompt_cta_rows(max_q_len * r.G, num_seqs, r.Hkv);
+  const int64_t work_units = (max_q_len * r.G + p.cta_rows - 1) / p.cta_rows * num_seqs * r.Hkv;
+  p.num_splits = prompt_plan(work_units, keys).splits;
   TORCH_CHECK(num_seqs <= 65535 && (int64_t)r.Hkv * p.num_splits <= 65535, "attention: launch grid too large");
-  torch::Tensor po, pl, ctr;
+  torch::Tensor po, pl, ctr;  // the join's counters belong to this call alone
   if (p.num_splits > 1) {
     const auto f32 = work.options().dtype(at::kFloat);
     po = torch::empty({T * r.Hq * p.num_splits * 128}, f32);
@@ -1316,9 +1367,7 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out_arg, const 
   int64_t keys = std::max<int64_t>(1, max_kv_len);
   if (window > 0) keys = std::min(keys, window + sinks + max_q_len);
   const int64_t rows = max_q_len * p.G;
-  // From 512 (token, head) rows, half of where the calls without a window and a 4-bit cache change kernels: 128 queries
-  // of 32 heads over 3200 keys 73 us by rows and 61 here (bf16: 119 and 46), 64 queries 46 and 59 (bf16 60 and 49).
-  if (max_q_len > 1 && attn_prefill_tc_use((int)D, 2 * T * p.G)) {
+  if (D == 128 && max_q_len > 1 && prompt_pays(q4, T, num_seqs, max_q_len, p.G, Hkv, PS, keys, page_ids.numel())) {
     attention_prompt(p, q4 ? nullptr : &kv, kv, scales, T, num_seqs, max_q_len, keys, page_ids.numel(), st);
     return out;
   }

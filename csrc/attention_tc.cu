@@ -751,6 +751,8 @@ static int attn_tc_mode() {
   return g_attn_tc >= 0 ? g_attn_tc : env_mode;
 }
 
+int attn_prefill_tc_mode() { return attn_tc_mode(); }
+
 // Prefill call of `rows` (token, head) rows with head dim D.
 bool attn_prefill_tc_use(int D, int64_t rows) {
   if (D != TC_D) return false;

@@ -81,6 +81,7 @@ torch::Tensor attention_rows(const c10::optional<torch::Tensor>& out, const torc
                              const torch::Tensor& seg_delta, const torch::Tensor& page_ids, const torch::Tensor& cos,
                              const torch::Tensor& sin, double scale, bool use_rope, int64_t num_seqs,
                              int64_t max_q_len, int64_t max_kv_len, int64_t window, int64_t sinks);
+int64_t attn_kv4_workspace_limit();
 torch::Tensor qkv_prepare_kv4(const torch::Tensor& qkv, const torch::Tensor& positions, const torch::Tensor& slots,
                               const torch::Tensor& codes, const torch::Tensor& scales,
                               const c10::optional<torch::Tensor>& q_norm, const c10::optional<torch::Tensor>& k_norm,
@@ -158,6 +159,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("seq_nsh") = py::none(), py::arg("shared_splits") = 0, py::arg("grp_max_q") = 0);
   m.def("attention_rows", &braid::attention_rows,
         "paged cascade attention of few rows over a bf16 or 4-bit cache, with an optional window and sinks");
+  m.def("attn_kv4_workspace_limit", &braid::attn_kv4_workspace_limit,
+        "largest bf16 workspace in bytes that an attention call over a 4-bit cache takes");
   m.def("qkv_prepare_kv4", &braid::qkv_prepare_kv4, "q/k norm, RoPE(k) and append to the 4-bit paged cache");
   m.def("kv4_read", &braid::kv4_read, "the values a 4-bit cache holds at the given slots");
   m.def("attn_prefill_tile_rows", &braid::attn_prefill_tile_rows,

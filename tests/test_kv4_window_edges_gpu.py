@@ -264,3 +264,99 @@ def test_v_steps_far_from_one(d, nq, exponent):
     cos, sin = _tables(d)
     got = ops.attention(q, layer, meta, cos, sin, d ** -0.5)
     check(got, dense64(q, unpack64(layer), meta, cos, sin, d ** -0.5, base=code8(layer)), ROWS4)
+
+
+# -------------------------------------------------------- choice of the kernel
+def _peak(call):
+    """(what the call gives, bytes that it held beyond that at its peak)"""
+    call()
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - base - out.numel() * out.element_size()
+
+
+@pytest.mark.parametrize("nq,n", [(2, 64), (3, 40)])
+def test_many_sequences_of_few_queries_take_no_workspace(nq, n):
+    """Rows of a sequence choose the kernel, not those of the batch: the pages are not read into bf16 for a few queries."""
+    d, G, hkv, ps, keys = 128, 4, 2, 16, 1000
+    pages = n * -(-keys // ps)
+    meta, T = make_plan([(nq, [(keys, 0, 0)])] * n, ps, pages, DEV)
+    cache, kv = _pool(4, pages, hkv, ps, d)
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    out, held = _peak(lambda: ops.attention(q, cache, meta, cos, sin, d ** -0.5))
+    check(out, dense64(q, kv, meta, cos, sin, d ** -0.5, base=code8(cache)), ROWS4)
+    assert held <= 1 << 20 < pages * ps * hkv * 512
+
+
+def test_a_shared_chunk_that_many_sequences_list_stays_within_the_workspace_limit():
+    """80 sequences of 32 queries over one cached chunk of 8192 tokens: its pages, listed 80 times, would take 2.7 GB."""
+    d, G, hkv, ps, nq, n, chunk = 128, 4, 8, 256, 32, 80, 8192
+    one, _ = make_plan([(nq, [(chunk, 0, 3), (nq, 0, 0)])], ps, 40, DEV)
+    layer = rand_layer4(40, hkv, ps, d, 0, DEV)
+    cat = lambda f, step: torch.cat([getattr(one, f)[:-1] + i * step for i in range(n)] + [getattr(one, f)[-1:] + (n - 1) * step])  # noqa: E731
+    many = ops.AttnMeta(num_seqs=n, max_q_len=nq, max_kv_len=one.max_kv_len, qo_indptr=cat("qo_indptr", nq),
+                        seg_indptr=cat("seg_indptr", 2), seg_page_indptr=cat("seg_page_indptr", one.page_ids.numel()),
+                        **{f: getattr(one, f).repeat(n) for f in ("positions", "seg_offset", "seg_len", "seg_pos0",
+                                                                  "seg_delta", "page_ids")})
+    limit = ext().attn_kv4_workspace_limit()
+    assert many.page_ids.numel() * ps * hkv * 512 > limit
+    q = _queries(nq, hkv * G, d)
+    cos, sin = _tables(d, 9000)
+    alone = ops.attention(q, layer, one, cos, sin, d ** -0.5)
+    check(alone, dense64(q, unpack64(layer), one, cos, sin, d ** -0.5, base=code8(layer)), TC4)
+    out, held = _peak(lambda: ops.attention(q.repeat(n, 1, 1), layer, many, cos, sin, d ** -0.5))
+    assert held <= limit + (1 << 28)
+    out = out.view(n, nq, -1)
+    assert all(torch.equal(out[i], out[0]) for i in range(n))
+    check(out[0], dense64(q, unpack64(layer), one, cos, sin, d ** -0.5, base=code8(layer)), TC4)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("G,hkv", [(4, 2), (1, 8), (16, 1)])
+def test_both_kernels_over_a_ragged_batch(bits, G, hkv):
+    """The kernel that is chosen and the one that is not, over one long prompt among short ones."""
+    d, ps = 128, 16
+    seqs = [(400, [(300, 2, 1), (400, 0, 0)])] + [(1 + i % 5, [(60 + 37 * i, 0, 0)]) for i in range(12)]
+    pages = 400
+    meta, T = make_plan(seqs, ps, pages, DEV)
+    cache, kv = _pool(bits, pages, hkv, ps, d)
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    window = 0 if bits == 4 else 250
+    ref = dense64(q, kv, meta, cos, sin, d ** -0.5, window, 2)
+    outs = {}
+    try:
+        for mode in (0, 1, -1):
+            ext().attn_select_prefill_tc(mode)
+            outs[mode] = ops.attention(q, cache, meta, cos, sin, d ** -0.5, window=window, sinks=2)
+            check(outs[mode], ref, TC4 if bits == 4 else TC16)
+    finally:
+        ext().attn_select_prefill_tc(-1)
+    assert torch.equal(outs[-1], outs[0]) or torch.equal(outs[-1], outs[1])
+
+
+def test_the_pool_leaves_room_for_the_workspace(tmp_path, monkeypatch):
+    from braidinfer_b200 import LLM
+    from braidinfer_b200.utils.synthetic import make_checkpoint
+    ck = make_checkpoint(str(tmp_path), "tiny-qwen3", seed=0, head_dim=128)
+    kw = dict(num_kvcache_blocks=32, kvcache_block_size=16, max_graph_batch=2)
+    llm = LLM(ck, **kw)
+    assert llm.model_runner.attention_workspace_bytes() == 0
+    llm.exit()
+    llm = LLM(ck, kv_cache_dtype="int4", **kw)
+    mr = llm.model_runner
+    limit = ext().attn_kv4_workspace_limit()
+    # the pages of one sequence and the padding one in the prefill graphs; of 256 sequences in eager steps, the limit
+    graph = (-(-mr.config.max_model_len // 16) + 17) * 16 * 2 * 512
+    assert mr.attention_workspace_bytes() == min(limit, 256 * graph) + graph
+    mr.config.num_kvcache_blocks = -1
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (120 << 30, 180 << 30))
+    pages = mr.auto_num_pages()
+    reserved = mr.attention_workspace_bytes()
+    monkeypatch.setattr(mr, "attention_workspace_bytes", lambda: 0)
+    assert abs((mr.auto_num_pages() - pages) * mr.kv_bytes_per_page() - reserved) <= mr.kv_bytes_per_page()
+    llm.exit()
