@@ -8,7 +8,8 @@ A layer is a :class:`KV4Layer` of two tensors,
   ``z``) for each group of 64 elements.
 
 An element stands for ``s * c + z``.  A group with least element ``a`` and
-largest ``b`` has ``s = bf16((b - a) / 15)``, ``z = bf16(a)`` and
+largest ``b`` has ``s = bf16((b - a) * r)`` with ``r`` the fp32 number next to
+1/15 and the product rounded to fp32 first, ``z = bf16(a)`` and
 ``c = round((x - z) / s)`` clamped to 0..15 (0 where ``s`` is 0), so a value is
 off by at most half a step plus what rounding ``s`` and ``z`` to bf16 shifts the
 ends of the range: ``|x' - x| <= s / 2 + 2**-8 * (|a| + |b|)``.  A group that
@@ -84,7 +85,8 @@ def kv4_pack_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     a, b = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
     fine = g.isfinite().all(-1, keepdim=True) & (b - a).isfinite()
     nan = torch.full_like(a, float("nan"))
-    s, z = torch.where(fine, (b - a) / 15, nan).bfloat16(), torch.where(fine, a, nan).bfloat16()
+    fifteenth = torch.tensor(1 / 15, dtype=torch.float32, device=a.device)  # a product, as on CUDA: not a division
+    s, z = torch.where(fine, (b - a) * fifteenth, nan).bfloat16(), torch.where(fine, a, nan).bfloat16()
     step = s.float()
     c = torch.where(fine & (step > 0), (g - z.float()) / torch.where(step > 0, step, torch.ones_like(step)),
                     torch.zeros_like(g))

@@ -2,7 +2,10 @@
 //   codes  uint8 [P, 2, Hkv, PS, D/2]      K (0) and V (1) rows of D 4-bit codes
 //   scales bf16  [P, 2, Hkv, PS, D/64, 2]  one (scale s, offset z) pair per group of 64 elements
 // and element x of a row stands for s * c + z.  A group with least element a
-// and largest b has s = bf16((b - a) / 15), z = bf16(a) and
+// and largest b has s = bf16((b - a) r) with r the fp32 number next to 1/15 (a
+// product costs less than a division and differs from it in the last fp32 bit at
+// most, so s only where the quotient lies that near to a border between two bf16
+// numbers), z = bf16(a) and
 // c = round((x - z) / s) clamped to 0..15 (0 where s is 0); a group that holds
 // a NaN or an infinity gets s = z = NaN, so every element of it reads as NaN.
 // A row of 128 elements takes 64 + 8 bytes instead of 256.

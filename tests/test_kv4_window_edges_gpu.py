@@ -360,3 +360,24 @@ def test_the_pool_leaves_room_for_the_workspace(tmp_path, monkeypatch):
     monkeypatch.setattr(mr, "attention_workspace_bytes", lambda: 0)
     assert abs((mr.auto_num_pages() - pages) * mr.kv_bytes_per_page() - reserved) <= mr.kv_bytes_per_page()
     llm.exit()
+
+
+# ------------------------------------------------------------------- append
+def test_append_gives_the_scales_of_the_cpu_form():
+    """Ranges whose fifteenth lies on or next to a border between two bf16 numbers: 15 t with t of 9 bits."""
+    d, ps, P = 64, 16, 16
+    t = torch.arange(257, 512, 2)
+    r = 15 * t
+    top = (r // 32 * 32).float()
+    x = torch.zeros(t.numel(), 3 * d)
+    x[:, 2 * d], x[:, 2 * d + 1] = top, top - r.float()  # largest and least of V, both of at most 8 bits
+    assert torch.equal(x.bfloat16().float(), x)
+    slots = torch.arange(t.numel(), dtype=torch.int32)
+    cos, sin = _tables(d)
+    held = []
+    for dev in ("cpu", DEV):
+        layer = ops.KV4Cache(1, P, 1, ps, d, device=dev)[0]
+        ops.qkv_prepare(x.bfloat16().to(dev), slots.to(dev), slots.to(dev), layer, 1, 1, d, cos.to(dev), sin.to(dev))
+        held.append(layer)
+    assert torch.equal(held[0].scales[:, 1], held[1].scales[:, 1].cpu())
+    assert torch.equal(held[0].codes[:, 1], held[1].codes[:, 1].cpu())
