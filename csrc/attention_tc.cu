@@ -787,11 +787,13 @@ void launch_attn_prefill_tc(const AttnParams& p, int num_seqs, int max_q_len, in
   }();
   const int poly = g_attn_poly >= 0 ? g_attn_poly : env_poly;
   auto go = [&](auto k, int br) {
-    static bool attr[16] = {};
+    static bool attr[64][16] = {};  // attributes are per device
+    int dev;
+    C10_CUDA_CHECK(cudaGetDevice(&dev));
     const int slot = (br == 64 ? 4 : 0) + (p.window > 0 ? 8 : poly == 2 ? 1 : poly == 4 ? 2 : 0);
-    if (!attr[slot]) {
+    if (!attr[dev & 63][slot]) {
       C10_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem::TOTAL));
-      attr[slot] = true;
+      attr[dev & 63][slot] = true;
     }
     launch_pdl(k, grid, dim3(TC_THREADS), TcSmem::TOTAL, st, make_tmap(p.kv, rows, TC_D, TC_D, br), p);
   };

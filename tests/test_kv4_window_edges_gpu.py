@@ -381,3 +381,24 @@ def test_append_gives_the_scales_of_the_cpu_form():
         held.append(layer)
     assert torch.equal(held[0].scales[:, 1], held[1].scales[:, 1].cpu())
     assert torch.equal(held[0].codes[:, 1], held[1].codes[:, 1].cpu())
+
+
+@pytest.mark.multigpu
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("nq", [1, 30, 300])
+def test_tensors_on_another_device_than_the_current_one(bits, nq):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs 2 GPUs")
+    d, ps, hkv, G, pages = 128, 16, 2, 4, 64
+    outs = []
+    for dev in ("cuda:0", "cuda:1"):
+        meta, T = make_plan([(nq, [(700, 0, 0)])], ps, pages, dev)
+        cache = rand_layer4(pages, hkv, ps, d, 0, "cpu")
+        cache = ops.KV4Layer(*(t.to(dev) for t in cache)) if bits == 4 else unpack64(cache).bfloat16().to(dev)
+        q = torch.randn(T, hkv * G, d, generator=torch.Generator().manual_seed(1)).bfloat16().to(dev)
+        cos, sin = ops.build_cos_sin(d, 1e4, 1024, device="cpu")
+        out = ops.attention(q, cache, meta, cos.to(dev), sin.to(dev), d ** -0.5, window=600)
+        assert out.device == torch.device(dev)
+        outs.append(out.cpu())
+        assert torch.cuda.current_device() == 0
+    assert torch.equal(*outs)
