@@ -1,7 +1,7 @@
 """4-bit and windowed attention on a GPU where launches, splits, values and batches end."""
 import pytest
 import torch
-from kv4_helpers import ROWS4, ROWS16, TC4, TC16, check, code8, dense64, make_plan, rand_layer4, unpack64
+from kv4_helpers import ROWS4, ROWS16, TC4, TC16, check, code8, dense64, make_plan, rand_layer4, tolerance, unpack64
 
 from braidinfer_b200 import ops
 from braidinfer_b200.ops._ext import ext
@@ -402,3 +402,76 @@ def test_tensors_on_another_device_than_the_current_one(bits, nq):
         outs.append(out.cpu())
         assert torch.cuda.current_device() == 0
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("count", [3, 64])
+@pytest.mark.parametrize("climb", [40, -6])
+def test_decode_with_scores_and_v_steps_that_move(d, count, climb):
+    """Decode rows whose scores climb by far more than 2^8 along the keys while V's steps climb by 2^40 or fall by 2^6:
+    maxima and the power of two of P move, in the instances for few (3 sequences) and for many CTAs."""
+    ps, hkv, G, pages = 16, 8, 1, 64 * 40
+    lens = [600 - 7 * i for i in range(count)]
+    meta, T = make_plan([(1, [(n, 0, 0)]) for n in lens], ps, pages, DEV)
+    layer = rand_layer4(pages, hkv, ps, d, 0, DEV)
+    part = torch.zeros(pages * ps, device=DEV)  # of every slot, how far along its sequence it lies
+    h = meta.host
+    largest = torch.zeros(T, hkv * G, d, dtype=torch.float64, device=DEV)
+    places = []
+    for b, n in enumerate(lens):
+        j = torch.arange(n, device=DEV)
+        at = h["page_ids"].to(DEV).long()[int(h["seg_page_indptr"][b]) + j // ps] * ps + j % ps
+        part[at] = j / n
+        places.append(at)
+    part = part.view(pages, 1, ps, 1, 1)
+    layer.scales[:, 0] = (layer.scales[:, 0].float() * (0.1 + 4 * part)).bfloat16()
+    layer.scales[:, 1] = (layer.scales[:, 1].float() * torch.exp2(climb * (part - int(climb > 0)))).bfloat16()
+    q = _queries(T, hkv * G, d)
+    cos, sin = _tables(d)
+    got = ops.attention(q, layer, meta, cos, sin, d ** -0.5, use_rope=False)
+    out, A, B = dense64(q, unpack64(layer), meta, cos, sin, d ** -0.5, use_rope=False, base=code8(layer))
+    # P s is held in fp16 against the largest step that the warp has met: below 2^-14 of it a rounding is 2^-25 of it,
+    # times a code of at most 8 from the middle, for each key; the weights sum to at least 1, and as many terms of up to A
+    # are summed in fp32
+    for b, at in enumerate(places):
+        step = layer.scales[at // ps, 1, :, at % ps][..., 0].double()  # [n, Hkv, D/64]
+        largest[b] = step.amax(0).amax(-1)[:, None].expand(hkv, d)
+    tol = tolerance(out, A, B, *ROWS4) + 600 * 2 ** -24 * A + 600 * 2 ** -22 * largest.view(T, -1)
+    assert ((got.double() - out).abs() <= tol).all()
+    # the bound says something: it is far below the outputs
+    assert (tol.norm(dim=-1) <= 0.1 * out.norm(dim=-1)).all()
+
+
+# -------------------------------------------------------------------- engine
+@pytest.mark.parametrize("extra", [dict(kv_cache_dtype="int4"), dict(sliding_window=100, attention_sinks=3),
+                                   dict(kv_cache_dtype="int4", sliding_window=100)])
+@pytest.mark.parametrize("n", [33, 190, 250])
+def test_engine_prefill_graphs_with_head_dim_128(extra, n, tmp_path, tcgen05):
+    """A prompt through a captured prefill, padded in tokens, segments and pages, beside a padding sequence, on the tcgen05
+    kernel and its workspace inside the graph: the K and V that it leaves are those of an eager step.  Layer 1's follow
+    from the attention of layer 0."""
+    from braidinfer_b200 import LLM, SamplingParams
+    from braidinfer_b200.utils.synthetic import make_checkpoint
+    ck = make_checkpoint(str(tmp_path), "tiny-qwen3", seed=0, head_dim=128)
+    prompts = [[(7 * i + 13 * j) % 1000 + 3 for j in range(n)] for i in range(3)]
+    held = []
+    for eager in (True, False):
+        llm = LLM(ck, num_kvcache_blocks=200, kvcache_block_size=16, max_graph_batch=2, enforce_eager=eager, **extra)
+        for p in prompts:  # each on pages of its own; the graph is captured by the first and replayed by the others
+            llm.generate([p], SamplingParams(temperature=0, max_tokens=1, ignore_eos=True))
+        assert eager or llm.model_runner.prefill_graphs
+        whole = llm.page_manager.kv_cache
+        if isinstance(whole, ops.KV4Cache):
+            held.append([unpack64(whole[i]) for i in range(2)])
+        else:
+            held.append([whole[i].double() for i in range(2)])
+        llm.exit()
+    scratch = 199
+    for layer, (a, b) in enumerate(zip(*held)):
+        a, b = (x[:scratch].movedim(3, 1).flatten(0, 1).flatten(1) for x in (a, b))  # a row per slot
+        used = a.norm(dim=-1) > 0
+        assert used.sum() >= 3 * n and torch.equal(used, b.norm(dim=-1) > 0)
+        # bf16 hidden states differ by a few roundings of 2^-9, 2^-7 in all; in 4 bits such a shift puts 1 in 40 elements
+        # on another code, a step (a fifteenth of the range, a third of the rms) off: 0.06 of the norm
+        far = (a - b).norm(dim=-1)[used] / a.norm(dim=-1)[used]
+        assert far.max() <= (2 ** -2 if "kv_cache_dtype" in extra else 2 ** -5), (layer, float(far.max()))
