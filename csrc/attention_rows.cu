@@ -34,12 +34,13 @@
 // overflow, below that, bits are lost.  With a bf16 cache the rotated query is
 // split into two bf16 terms (hi + lo, 16 bits) and P is rounded to bf16 once.
 //
-// Measured on a B200 (GPU time, head_dim 128): a 4-bit cache is read at 4.0-4.2
-// TB/s with every SM busy and is bound by issue: taking the codes apart (K 40, V
-// 48 logic instructions for 16 keys, on a pipe of half rate) and the softmax; the
-// ring alone, without consumers, brings 6.7 TB/s.  A bf16 cache (32 windowed
-// requests) is read at 6.2 TB/s.  A call's fixed time is about 6.5 us: four
-// dependent reads of the plan, the first tile, one step, the join.
+// Measured on a B200 (GPU time, head_dim 128): a 4-bit cache is read at 4.0-4.3
+// TB/s with every CTA slot busy.  Neither DRAM nor a pipe is full there (ALU pipe
+// 45%, where the codes are taken apart, issue 51%): chains of dependent
+// instructions on 2 to 3.5 warps a scheduler bound it, and registers the warps.
+// A bf16 cache (32 windowed requests) is read at 6.2 TB/s.  A call's fixed time
+// is about 6.5 us: four dependent reads of the plan, the first tile, one step,
+// the join.
 //
 // The keys that a tile can see (the sink part and the window part of every
 // segment) are split over the CTAs of a thread-block cluster, whose partial
@@ -645,12 +646,12 @@ __global__ void __launch_bounds__(ROWS_THREADS, OCC) attn_rows_kernel(const __gr
 #pragma unroll
       for (int c = 0; c < 2; ++c) th[nt][c] = m[nt][c] == ROWS_M0 ? ROWS_M0 : (m[nt][c] + 8.f) / hm[nt][c];
   };
-  // The first segment's delta (most plans have one for all) while the first copies are under way.
   uint32_t m8[4];  // opaque, or the compiler would rebuild them for every use
   asm volatile("mov.b32 %0, %2; mov.b32 %1, %3;" : "=r"(m8[0]), "=r"(m8[1]) : "n"(NIB_LO_M8), "n"(NIB_HI_M8));
   m8[2] = m8[0];
   m8[3] = m8[1];
   bool ok = true;
+  // the first segment's delta (most plans have one for all) while the first copies are under way
   int built = nseg > 0 ? segs.delta[0] : 0;
   if (warp < ROWS_WARPS) build(built, xq);
   int st = 0, ph = 0;
@@ -1165,7 +1166,7 @@ static void launch_rows(RowsParams& p, int64_t pool_rows, int64_t num_seqs, int6
 // Calls of many rows a sequence (head_dim 128): the tcgen05 prefill kernel of attention_tc.cu with the window.  A 4-bit
 // cache is first read into a bf16 workspace, page by page as the plan lists them: one more rounding of K and V to bf16,
 // and 2 + 0.56 bytes an element once per call, against the whole prompt's products (4000 tokens of Llama-3-8B heads: 8 of
-// 190 us).
+// 196 us).
 int attn_prefill_tc_mode();
 int attn_prefill_tc_rows();
 int attn_prefill_tc_min_rows();
@@ -1207,10 +1208,10 @@ int64_t attn_kv4_workspace_limit() { return PROMPT_WORKSPACE; }
 //   queries x sequences over keys    4-bit cache        bf16 cache
 //    64 x 1 over  3200                41    56           55    46
 //   128 x 1 over  3200                67    60          108    44
-//     2 x 64 over 3200                87   447          135   224
+//     2 x 64 over 3200                87   450          135   230
 //    16 x 16 over 3200               131   120          223    61
 //    64 x 16 over 3200               453   133          748    73
-//    32 x 1 over 12000                68    85           99    63
+//    32 x 1 over 12000                70    88           99    63
 // Sequences of unequal length count by their rows together, a tile more for each.
 // A prompt of 512 rows takes the tcgen05 kernel also where that is up to 20 us slower (512 rows over 600 keys in 4 bits:
 // 21 and 30), so that prompts round alike whatever their length.

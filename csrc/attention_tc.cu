@@ -33,8 +33,8 @@
 // workspace) walk two intervals per segment, the sink part and the window part
 // of what the CTA's rows see, so keys behind every row's window are not loaded;
 // V rows outside the interval are zeroed before P V (P is 0 there, but the slots
-// may hold NaN).  Prompts of 3500 and 4096 tokens, window 1024: 246 us on a B200
-// (465 TFLOP/s of visible pairs; a 256-row CTA covers its window and 64 tokens
+// may hold NaN).  Prompts of 3500 and 4096 tokens, window 1024: 248 us on a B200
+// (462 TFLOP/s of visible pairs; a 256-row CTA covers its window and 64 tokens
 // more, and the sinks take a tile of their own).
 // Replaces the reference's per-page Triton online-softmax calls
 // (braidinfer/kernels/online_softmax.py:15-214) on the prefill side.

@@ -5,8 +5,8 @@
 // token's slot.  Everything from the bf16 input to the code is fp32; the only
 // roundings are those the format defines and, for a normalised q, one to bf16.
 // Measured on a B200: 8191 tokens of 16 query and 8 KV heads of 128 with norms
-// 40 us (110 MB: 2.7 TB/s; bound by issue, half of it norm, rotation and
-// quantisation of the K and V rows), read-back of the same tokens 12 us.
+// 40 us (110 MB: 2.7 TB/s; bound by issue, 76% of cycles: norm, rotation and
+// quantisation), read-back of the same tokens 12 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
