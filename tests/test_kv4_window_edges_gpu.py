@@ -293,8 +293,8 @@ def test_many_sequences_of_few_queries_take_no_workspace(nq, n):
 
 
 def test_a_shared_chunk_that_many_sequences_list_stays_within_the_workspace_limit():
-    """80 sequences of 32 queries over one cached chunk of 8192 tokens: its pages, listed 80 times, would take 2.7 GB."""
-    d, G, hkv, ps, nq, n, chunk = 128, 4, 8, 256, 32, 80, 8192
+    """160 sequences of 32 queries over one cached chunk of 8192 tokens: its pages, listed 160 times, would take 5.5 GB."""
+    d, G, hkv, ps, nq, n, chunk = 128, 4, 8, 256, 32, 160, 8192
     one, _ = make_plan([(nq, [(chunk, 0, 3), (nq, 0, 0)])], ps, 40, DEV)
     layer = rand_layer4(40, hkv, ps, d, 0, DEV)
     cat = lambda f, step: torch.cat([getattr(one, f)[:-1] + i * step for i in range(n)] + [getattr(one, f)[-1:] + (n - 1) * step])  # noqa: E731
