@@ -475,3 +475,18 @@ def test_engine_prefill_graphs_with_head_dim_128(extra, n, tmp_path, tcgen05):
         # on another code, a step (a fifteenth of the range, a third of the rms) off: 0.06 of the norm
         far = (a - b).norm(dim=-1)[used] / a.norm(dim=-1)[used]
         assert far.max() <= (2 ** -2 if "kv_cache_dtype" in extra else 2 ** -5), (layer, float(far.max()))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("d,nq", [(64, 5), (128, 5), (128, 300)])
+def test_queries_within_wider_rows(bits, d, nq):
+    """Queries as the append returns them without a q norm, columns of the QKV rows, in every kernel."""
+    hkv, G, ps, pages = 2, 4, 16, 64
+    meta, T = make_plan([(nq, [(300, 1, 0), (nq, 0, 0)]), (1, [(33, 0, 0)])], ps, pages, DEV)
+    cache, _ = _pool(bits, pages, hkv, ps, d)
+    wide = torch.randn(T, (G + 2) * hkv * d + 8, device=DEV, generator=_gen(2)).bfloat16()
+    q = wide[:, 8:8 + G * hkv * d].unflatten(1, (G * hkv, d))
+    assert not q.is_contiguous()
+    cos, sin = _tables(d)
+    run = lambda q: ops.attention(q, cache, meta, cos, sin, d ** -0.5, window=250, sinks=2)  # noqa: E731
+    assert torch.equal(run(q), run(q.contiguous()))
